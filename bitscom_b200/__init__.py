@@ -17,6 +17,8 @@ DDP::
 
 from .api import LowBitGroup
 from .lowbit_backend import backend_options, is_extension_available, register_lowbit_backend
+from .ops.attention import AttentionMask, attention, attention_mask
+from .ops.rotary import qk_norm_rotary, rotary_frequencies
 from .parallel.comm import Communicator
 from .parallel.fsdp import LowBitShardedDP
 from .parallel.graphs import GraphedStep
@@ -59,6 +61,11 @@ __all__ = [
     "roundtrip_tensor",
     "ef_roundtrip",
     "validate_bitwidth",
+    "AttentionMask",
+    "attention",
+    "attention_mask",
+    "qk_norm_rotary",
+    "rotary_frequencies",
 ]
 
 __version__ = "0.1.0"

@@ -4,6 +4,7 @@
 //   * the standalone quantisation ops (reference-compatible layout and
 //     semantics; reference bindings: cpp/src/lowbit_cuda_bindings.cpp:25-56),
 //     all launched on the caller's current CUDA stream and free of host syncs;
+//   * the attention operators (ops/attention_ops.cpp);
 //   * LowBitComm, the fused low-bit collective runtime;
 //   * the `lowbit` c10d backend (registered from backend/process_group_lowbit.cpp).
 #include <ATen/cuda/CUDAContext.h>
@@ -17,6 +18,7 @@
 
 #include "backend/process_group_lowbit.h"
 #include "kernels/launchers.h"
+#include "ops/attention_ops.h"
 #include "runtime/comm.h"
 
 namespace bitscom_b200 {
@@ -332,5 +334,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_property_readonly("timing", &LowBitComm::timing)
       .def("reset_stats", &LowBitComm::reset_stats);
 
+  register_attention_bindings(m);
   register_backend_bindings(m);
 }

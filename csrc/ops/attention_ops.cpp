@@ -1,0 +1,347 @@
+// Argument checks and Python bindings of the attention operators: masked
+// attention (forward, backward, mask plans) and the per-head norm with
+// rotation.  Every launch is on the caller's current stream of the tensors'
+// device; workspaces come from the caching allocator on that stream.
+#include "ops/attention_ops.h"
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "kernels/attention.h"
+#include "kernels/qk_norm_rotary.h"
+
+namespace bitscom_b200 {
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+DType float_type(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kF32;
+    case at::kBFloat16: return kBF16;
+    case at::kHalf: return kF16;
+    default:
+      TORCH_CHECK_TYPE(false, "bitscom: ", name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+bool has(const OptTensor& t) { return t && t->defined(); }
+
+void same_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), "bitscom: ", name, " is on ", t.device(), ", expected ", like.device());
+}
+
+int int_bytes(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "bitscom: ", name,
+                   " must be int32 or int64, got ", t.scalar_type());
+  return t.scalar_type() == at::kLong ? 8 : 4;
+}
+
+cudaStream_t stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// ---------------------------------------------------------------------------
+// Attention
+// ---------------------------------------------------------------------------
+
+// A [B, H, S, D] tensor as the kernels read it, copied when its last
+// dimension is not contiguous.
+at::Tensor rows_of(const at::Tensor& t) { return t.stride(3) == 1 || t.size(3) <= 1 ? t : t.contiguous(); }
+
+AttnTensor view_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+
+// New [B, H, S, D] tensor laid out [B, S, H, D], the order in which projections leave and take it.
+at::Tensor tokens_first(const at::Tensor& like) {
+  return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2);
+}
+
+void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+  TORCH_CHECK_VALUE(q.is_cuda() && k.is_cuda() && v.is_cuda(), "bitscom: q, k and v must be CUDA tensors");
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
+                    "bitscom: q, k and v must be [batch, heads, length, head size]");
+  float_type(q, "q");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                   "bitscom: q, k and v must have one dtype, got ", q.scalar_type(), ", ", k.scalar_type(), " and ",
+                   v.scalar_type());
+  same_device(k, q, "k");
+  same_device(v, q, "v");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "bitscom: k and v must have one shape, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(3) == q.size(3), "bitscom: q ", q.sizes(), " and k ", k.sizes(),
+                    " must agree in batch and head size");
+  TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) % k.size(1) == 0, "bitscom: ", q.size(1),
+                    " query heads are not a multiple of ", k.size(1), " key heads");
+  TORCH_CHECK_VALUE(q.size(3) >= 1 && q.size(3) <= 256, "bitscom: head size must be 1 to 256, got ", q.size(3));
+  TORCH_CHECK_VALUE(q.size(0) <= 65535 && q.size(1) <= 65535, "bitscom: at most 65535 batch entries and heads");
+  TORCH_CHECK_VALUE(q.size(2) < (1 << 30) && k.size(2) < (1 << 30), "bitscom: lengths must be below 2^30");
+}
+
+AttnParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
+                     const OptTensor& slopes, bool causal, double scale, double cap) {
+  AttnParams p{};
+  p.q = view_of(q);
+  p.k = view_of(k);
+  p.v = view_of(v);
+  p.b = static_cast<int>(q.size(0));
+  p.hq = static_cast<int>(q.size(1));
+  p.hk = static_cast<int>(k.size(1));
+  p.sq = static_cast<int>(q.size(2));
+  p.sk = static_cast<int>(k.size(2));
+  p.d = static_cast<int>(q.size(3));
+  p.causal = causal;
+  p.scale = static_cast<float>(scale);
+  p.cap = static_cast<float>(cap);
+  p.splits = 1;
+  p.dt = float_type(q, "q");
+  if (has(slopes)) {
+    same_device(*slopes, q, "slopes");
+    TORCH_CHECK_TYPE(slopes->scalar_type() == at::kFloat, "bitscom: slopes must be float32");
+    TORCH_CHECK_VALUE(slopes->dim() == 1 && slopes->size(0) == q.size(1) && slopes->is_contiguous(),
+                      "bitscom: slopes must be a contiguous vector of one value for each of the ", q.size(1),
+                      " query heads");
+    p.slopes = slopes->data_ptr<float>();
+  }
+  if (has(plan)) {
+    same_device(*plan, q, "mask");
+    TORCH_CHECK_VALUE(plan->scalar_type() == at::kInt && plan->is_contiguous() &&
+                          plan->numel() == PlanView::words(p.b, p.sq, p.sk),
+                      "bitscom: the mask was built for other sizes");
+    p.plan = PlanView::of(plan->data_ptr<int>(), p.b, p.sq, p.sk);
+  }
+  return p;
+}
+
+at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, bool causal, int64_t batch, int64_t q_len,
+                          int64_t k_len) {
+  const at::Tensor& like = has(documents) ? *documents : *prefix;
+  TORCH_CHECK_VALUE(like.is_cuda(), "bitscom: documents and prefix must be CUDA tensors");
+  TORCH_CHECK_VALUE(batch >= 0 && batch <= 65535 && q_len >= 0 && k_len >= 0 && q_len < (1 << 30) && k_len < (1 << 30),
+                    "bitscom: batch must be at most 65535, lengths below 2^30");
+  int ids_bytes = 4, prefix_bytes = 4;
+  if (has(documents)) {
+    ids_bytes = int_bytes(*documents, "documents");
+    TORCH_CHECK_VALUE(documents->dim() == 2 && documents->size(0) == batch && documents->size(1) == k_len,
+                      "bitscom: documents must be [", batch, ", ", k_len, "] (batch, key length), got ",
+                      documents->sizes());
+  }
+  if (has(prefix)) {
+    prefix_bytes = int_bytes(*prefix, "prefix");
+    same_device(*prefix, like, "prefix");
+    TORCH_CHECK_VALUE(causal, "bitscom: a prefix needs a causal mask");
+    TORCH_CHECK_VALUE(prefix->dim() == 1 && prefix->size(0) == batch, "bitscom: prefix must be [", batch, "], got ",
+                      prefix->sizes());
+  }
+  c10::cuda::CUDAGuard g(like.device());
+  const at::Tensor pre = has(prefix) ? prefix->contiguous() : at::Tensor();
+  auto plan = at::empty({PlanView::words(batch, q_len, k_len)}, like.options().dtype(at::kInt));
+  if (plan.numel() == 0) return plan;
+  launch::attention_plan(has(documents) ? documents->data_ptr() : nullptr, ids_bytes,
+                         has(documents) ? documents->stride(0) : 0, has(documents) ? documents->stride(1) : 0,
+                         pre.defined() ? pre.data_ptr() : nullptr, prefix_bytes, causal, static_cast<int>(batch),
+                         static_cast<int>(q_len), static_cast<int>(k_len),
+                         PlanView::of(plan.data_ptr<int>(), batch, q_len, k_len), stream_of(like));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return plan;
+}
+
+// Returns (out, log-sums); the log-sums only when the backward pass wants them.
+std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q_in, const at::Tensor& k_in,
+                                                     const at::Tensor& v_in, const OptTensor& plan,
+                                                     const OptTensor& slopes, bool causal, double scale, double cap,
+                                                     bool want_lse) {
+  check_qkv(q_in, k_in, v_in);
+  c10::cuda::CUDAGuard g(q_in.device());
+  const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
+  AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
+  auto out = tokens_first(q);
+  at::Tensor lse;
+  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return {out, lse};
+  if (p.sk == 0) {
+    out.zero_();
+    if (want_lse) lse.fill_(std::numeric_limits<float>::infinity());
+    return {out, lse};
+  }
+  p.o = view_of(out);
+  p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  launch::attention_simt_forward(p, stream_of(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
+    const at::Tensor& dout_in, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+    const at::Tensor& out, const at::Tensor& lse, const OptTensor& plan, const OptTensor& slopes, bool causal,
+    double scale, double cap) {
+  check_qkv(q_in, k_in, v_in);
+  same_device(dout_in, q_in, "the output's gradient");
+  c10::cuda::CUDAGuard g(q_in.device());
+  const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
+  const auto dout = rows_of(dout_in.to(q.scalar_type()));
+  TORCH_CHECK_VALUE(dout.sizes() == q.sizes() && out.sizes() == q.sizes(), "bitscom: the output's gradient must be ",
+                    q.sizes());
+  auto dq = tokens_first(q), dk = tokens_first(k), dv = tokens_first(v);
+  if (q.numel() == 0 || k.numel() == 0) {
+    dq.zero_();
+    dk.zero_();
+    dv.zero_();
+    return {dq, dk, dv};
+  }
+  AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
+  auto delta = at::empty_like(lse);
+  p.o = view_of(out);
+  p.dout = view_of(dout);
+  p.dq = view_of(dq);
+  p.dk = view_of(dk);
+  p.dv = view_of(dv);
+  p.lse = lse.data_ptr<float>();
+  p.delta = delta.data_ptr<float>();
+  launch::attention_simt_backward(p, stream_of(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dv};
+}
+
+// ---------------------------------------------------------------------------
+// Norm of queries and keys with rotation
+// ---------------------------------------------------------------------------
+
+RotaryTensor heads_of(const at::Tensor& t) {
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), static_cast<int>(t.size(2))};
+}
+
+at::Tensor gains_of(const OptTensor& w, const at::Tensor& like, const char* name) {
+  if (!has(w)) return {};
+  same_device(*w, like, name);
+  float_type(*w, name);
+  TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == like.size(3), "bitscom: ", name, " must be [", like.size(3), "], got ",
+                    w->sizes());
+  return w->to(at::kFloat).contiguous();
+}
+
+struct RotaryCall {
+  at::Tensor q, k, wq, wk, freq;
+  RotaryParams p{};
+};
+
+RotaryCall rotary_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq, const OptTensor& wq,
+                       const OptTensor& wk, const OptTensor& positions, double eps, bool interleaved) {
+  TORCH_CHECK_VALUE(q.is_cuda() && k.is_cuda(), "bitscom: q and k must be CUDA tensors");
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4, "bitscom: q and k must be [batch, length, heads, head size]");
+  RotaryCall c;
+  c.p.dt = float_type(q, "q");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "bitscom: q and k must have one dtype, got ", q.scalar_type(),
+                   " and ", k.scalar_type());
+  same_device(k, q, "k");
+  TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3), "bitscom: q ", q.sizes(),
+                    " and k ", k.sizes(), " must agree in batch, length and head size");
+  const int64_t d = q.size(3);
+  TORCH_CHECK_VALUE(d >= 1 && d <= launch::kRotaryMaxDim, "bitscom: head size must be 1 to ", launch::kRotaryMaxDim,
+                    ", got ", d);
+  TORCH_CHECK_VALUE(q.size(0) * q.size(1) < (int64_t(1) << 31), "bitscom: at most 2^31 - 1 tokens");
+  TORCH_CHECK_VALUE(q.size(2) + k.size(2) <= 65535, "bitscom: at most 65535 heads");
+  same_device(freq, q, "frequencies");
+  TORCH_CHECK_TYPE(freq.is_floating_point(), "bitscom: frequencies must be floating point");
+  TORCH_CHECK_VALUE(freq.dim() == 1 && 2 * freq.size(0) <= d, "bitscom: frequencies must be a vector of at most ", d / 2,
+                    " values, got ", freq.sizes());
+  c.q = q.stride(3) == 1 || d == 1 ? q : q.contiguous();
+  c.k = k.stride(3) == 1 || d == 1 ? k : k.contiguous();
+  c.wq = gains_of(wq, q, "q_weight");
+  c.wk = gains_of(wk, k, "k_weight");
+  c.freq = freq.to(at::kDouble).contiguous();
+  RotaryParams& p = c.p;
+  p.q = heads_of(c.q);
+  p.k = heads_of(c.k);
+  p.wq = c.wq.defined() ? c.wq.data_ptr<float>() : nullptr;
+  p.wk = c.wk.defined() ? c.wk.data_ptr<float>() : nullptr;
+  p.freq = c.freq.data_ptr<double>();
+  if (has(positions)) {
+    same_device(*positions, q, "positions");
+    p.pos_bytes = int_bytes(*positions, "positions");
+    const bool row = positions->dim() == 1;
+    TORCH_CHECK_VALUE((row || positions->dim() == 2) && positions->size(-1) == q.size(1) &&
+                          (row || positions->size(0) == q.size(0)),
+                      "bitscom: positions must be [", q.size(1), "] or [", q.size(0), ", ", q.size(1), "], got ",
+                      positions->sizes());
+    p.positions = positions->data_ptr();
+    p.pos_sb = row ? 0 : positions->stride(0);
+    p.pos_ss = positions->stride(-1);
+  }
+  p.tokens = q.size(0) * q.size(1);
+  p.s = static_cast<unsigned>(q.size(1));
+  p.d = static_cast<int>(d);
+  p.rotated = static_cast<int>(2 * freq.size(0));
+  p.interleaved = interleaved;
+  p.eps = static_cast<float>(eps);
+  return c;
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
+                                                  const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
+                                                  double eps, bool interleaved) {
+  RotaryCall c = rotary_call(q, k, freq, wq, wk, positions, eps, interleaved);
+  c10::cuda::CUDAGuard g(q.device());
+  auto oq = at::empty(q.sizes(), q.options()), ok = at::empty(k.sizes(), k.options());
+  c.p.oq = heads_of(oq);
+  c.p.ok = heads_of(ok);
+  launch::qk_norm_rotary_forward(c.p, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, stream_of(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {oq, ok};
+}
+
+// Returns (dq, dk, dw [2, D] fp32 or undefined).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rotary_backward(const at::Tensor& gq_in, const at::Tensor& gk_in,
+                                                               const at::Tensor& q, const at::Tensor& k,
+                                                               const at::Tensor& freq, const OptTensor& wq,
+                                                               const OptTensor& wk, const OptTensor& positions,
+                                                               double eps, bool interleaved, bool want_dw) {
+  RotaryCall c = rotary_call(q, k, freq, wq, wk, positions, eps, interleaved);
+  c10::cuda::CUDAGuard g(q.device());
+  same_device(gq_in, q, "the gradient of q");
+  same_device(gk_in, q, "the gradient of k");
+  TORCH_CHECK_VALUE(gq_in.sizes() == q.sizes() && gk_in.sizes() == k.sizes(), "bitscom: gradients must be ", q.sizes(),
+                    " and ", k.sizes());
+  const auto fit = [&](const at::Tensor& t) {
+    auto x = t.to(q.scalar_type());
+    return x.stride(3) == 1 || x.size(3) == 1 ? x : x.contiguous();
+  };
+  const auto gq = fit(gq_in), gk = fit(gk_in);
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  auto dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+  c.p.oq = heads_of(dq);
+  c.p.ok = heads_of(dk);
+  c.p.gq = heads_of(gq);
+  c.p.gk = heads_of(gk);
+  at::Tensor dw, partial;
+  const auto f32 = q.options().dtype(at::kFloat);
+  if (want_dw) {
+    if (c.p.tokens == 0) {
+      dw = at::zeros({2, q.size(3)}, f32);
+    } else {
+      dw = at::empty({2, q.size(3)}, f32);
+      partial = at::empty({launch::qk_norm_rotary_blocks(c.p, sms), 2, q.size(3)}, f32);
+      c.p.partial = partial.data_ptr<float>();
+    }
+  }
+  launch::qk_norm_rotary_backward(c.p, sms, want_dw ? dw.data_ptr<float>() : nullptr, stream_of(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dw};
+}
+
+}  // namespace
+
+void register_attention_bindings(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.def("attention_plan", &attention_plan, py::arg("documents"), py::arg("prefix"), py::arg("causal"), py::arg("batch"),
+        py::arg("q_len"), py::arg("k_len"));
+  m.def("attention_forward", &attention_forward, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"),
+        py::arg("slopes"), py::arg("causal"), py::arg("scale"), py::arg("cap"), py::arg("want_lse"));
+  m.def("attention_backward", &attention_backward, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("out"), py::arg("lse"), py::arg("plan"), py::arg("slopes"), py::arg("causal"), py::arg("scale"),
+        py::arg("cap"));
+  m.def("rotary_forward", &rotary_forward, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
+        py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
+  m.def("rotary_backward", &rotary_backward, py::arg("gq"), py::arg("gk"), py::arg("q"), py::arg("k"), py::arg("freq"),
+        py::arg("wq"), py::arg("wk"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"), py::arg("want_dw"));
+}
+
+}  // namespace bitscom_b200

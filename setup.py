@@ -21,9 +21,13 @@ SOURCES = [
     "csrc/bindings.cpp",
     "csrc/runtime/comm.cpp",
     "csrc/backend/process_group_lowbit.cpp",
+    "csrc/ops/attention_ops.cpp",
     "csrc/kernels/quant_kernels.cu",
     "csrc/kernels/lowbit_coll.cu",
     "csrc/kernels/noalloc_allreduce.cu",
+    "csrc/kernels/attention_mask.cu",
+    "csrc/kernels/attention_simt.cu",
+    "csrc/kernels/qk_norm_rotary.cu",
 ]
 
 NVCC_FLAGS = [
