@@ -103,16 +103,16 @@ def attention_mask(
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan, slopes, causal, scale, cap):
-        out, lse = _ext._C.attention_forward(q, k, v, plan, slopes, causal, scale, cap, True)
-        ctx.save_for_backward(q, k, v, out, lse, plan, slopes)
+        out, lse, lo = _ext._C.attention_forward(q, k, v, plan, slopes, causal, scale, cap, True)
+        ctx.save_for_backward(q, k, v, out, lse, lo, plan, slopes)
         ctx.rest = (causal, scale, cap)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, plan, slopes = ctx.saved_tensors
-        dq, dk, dv = _ext._C.attention_backward(dout, q, k, v, out, lse, plan, slopes, *ctx.rest)
+        q, k, v, out, lse, lo, plan, slopes = ctx.saved_tensors
+        dq, dk, dv = _ext._C.attention_backward(dout, q, k, v, out, lse, lo, plan, slopes, *ctx.rest)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -143,7 +143,7 @@ def attention(
             several calls; ``mask`` replaces ``causal``, ``documents``, ``prefix``.
         softcap: cap of the scores (> 0), None for none.
         slopes: ``[heads]`` distance slopes (not differentiated).
-        scale: factor of ``q.k``, default ``head size ** -0.5``.
+        scale: factor of ``q.k`` (> 0), default ``head size ** -0.5``.
 
     Returns ``[batch, heads, q_len, head size]`` in q's dtype (stored
     ``[batch, q_len, heads, head size]``).  Rows that see no key are zero, with
@@ -156,6 +156,8 @@ def attention(
     """
     if softcap is not None and not softcap > 0:
         raise ValueError(f"softcap must be positive, got {softcap}")
+    if scale is not None and not scale > 0:
+        raise ValueError(f"scale must be positive, got {scale}")
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention does not differentiate slopes: detach them")
     if torch.is_autocast_enabled(q.device.type):

@@ -51,6 +51,7 @@ struct AttnTensor {  // [B, H, S, D] with D contiguous; strides in elements
 
 struct AttnParams {
   AttnTensor q, k, v, o, dout, dq, dk, dv;
+  AttnTensor lo;  // o minus its rounding to the tensors' type, laid out like o (null: not kept)
   float* lse;    // [B][Hq][Sq] log2 of the softmax denominator, +inf for a row without keys
   float* delta;  // [B][Hq][Sq] sum_d dout * o (backward)
   const float* slopes;  // [Hq] or null
@@ -76,6 +77,16 @@ void attention_plan(const void* ids, int ids_bytes, int64_t ids_sb, int64_t ids_
 // Elementary form in fp32 arithmetic for every type and head size up to 256.
 void attention_simt_forward(const AttnParams& p, cudaStream_t s);
 void attention_simt_backward(const AttnParams& p, cudaStream_t s);
+
+// Tensor-core form: fp16 and bf16, head sizes up to 128 that are multiples of 8,
+// rows on 16-byte boundaries.  The caller sets p.splits / split_tiles from attention_tc_splits and
+// allocates part_o / part_lse when there are several.
+void attention_tc_splits(const AttnParams& p, int sms, int* splits, int* split_tiles);
+cudaError_t attention_tc_forward(const AttnParams& p, cudaStream_t s);
+
+// 0, or 1 once a wait of a tensor-core kernel on the current device ran out (its
+// outputs are NaN then); `reset` clears it.  Waits for the device.
+int attention_status(bool reset);
 
 }  // namespace launch
 }  // namespace bitscom_b200

@@ -45,11 +45,29 @@ cudaStream_t stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStr
 // Attention
 // ---------------------------------------------------------------------------
 
-// A [B, H, S, D] tensor as the kernels read it, copied when its last
-// dimension is not contiguous.
-at::Tensor rows_of(const at::Tensor& t) { return t.stride(3) == 1 || t.size(3) <= 1 ? t : t.contiguous(); }
+// Whether the tensor-core kernels take these tensors (other forms: attention_simt.cu).
+bool for_tensor_cores(const at::Tensor& q) {
+  return q.scalar_type() != at::kFloat && q.size(3) % 8 == 0 && q.size(3) <= 128;
+}
 
-AttnTensor view_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+// A [B, H, S, D] tensor as the kernels read it: copied when its last dimension
+// is not contiguous, and for the tensor maps of the tensor-core kernels also
+// when a row does not start on a 16-byte boundary or a dimension is expanded.
+at::Tensor rows_of(const at::Tensor& t) {
+  bool fits = t.stride(3) == 1 || t.size(3) <= 1;
+  if (fits && for_tensor_cores(t)) {
+    fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
+  }
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Strides of dimensions of one entry are never used, and may be anything: a tensor map wants them to be legal.
+AttnTensor view_of(const at::Tensor& t) {
+  const int64_t any = (t.size(3) + 7) / 8 * 8;
+  const auto stride = [&](int i) { return t.size(i) <= 1 ? any : t.stride(i); };
+  return {t.data_ptr(), stride(0), stride(1), stride(2)};
+}
 
 // New [B, H, S, D] tensor laid out [B, S, H, D], the order in which projections leave and take it.
 at::Tensor tokens_first(const at::Tensor& like) {
@@ -144,34 +162,51 @@ at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, b
   return plan;
 }
 
-// Returns (out, log-sums); the log-sums only when the backward pass wants them.
-std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q_in, const at::Tensor& k_in,
-                                                     const at::Tensor& v_in, const OptTensor& plan,
-                                                     const OptTensor& slopes, bool causal, double scale, double cap,
-                                                     bool want_lse) {
+// Returns (out, log-sums, out's rounding); the last two only when the backward pass wants them.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tensor& q_in, const at::Tensor& k_in,
+            const at::Tensor& v_in, const OptTensor& plan,
+                                                                 const OptTensor& slopes, bool causal, double scale,
+                                                                 double cap, bool want_lse) {
   check_qkv(q_in, k_in, v_in);
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   auto out = tokens_first(q);
-  at::Tensor lse;
-  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-  if (out.numel() == 0) return {out, lse};
+  at::Tensor lse, lo;
+  const auto f32 = q.options().dtype(at::kFloat);
+  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, f32);
+  if (out.numel() == 0) return {out, lse, lo};
   if (p.sk == 0) {
     out.zero_();
     if (want_lse) lse.fill_(std::numeric_limits<float>::infinity());
-    return {out, lse};
+    return {out, lse, lo};
   }
   p.o = view_of(out);
   p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
-  launch::attention_simt_forward(p, stream_of(q));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {out, lse};
+  if (for_tensor_cores(q)) {
+    if (want_lse) {
+      lo = tokens_first(q);
+      p.lo = view_of(lo);
+    }
+    launch::attention_tc_splits(p, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.splits, &p.split_tiles);
+    at::Tensor part_o, part_lse;
+    if (p.splits > 1) {
+      part_o = at::empty({p.splits, q.size(0), q.size(1), q.size(2), q.size(3)}, f32);
+      part_lse = at::empty({p.splits, q.size(0), q.size(1), q.size(2)}, f32);
+      p.part_o = part_o.data_ptr<float>();
+      p.part_lse = part_lse.data_ptr<float>();
+    }
+    C10_CUDA_CHECK(launch::attention_tc_forward(p, stream_of(q)));
+  } else {
+    launch::attention_simt_forward(p, stream_of(q));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return {out, lse, lo};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     const at::Tensor& dout_in, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-    const at::Tensor& out, const at::Tensor& lse, const OptTensor& plan, const OptTensor& slopes, bool causal,
+    const at::Tensor& out, const at::Tensor& lse, const OptTensor& lo, const OptTensor& plan, const OptTensor& slopes, bool causal,
     double scale, double cap) {
   check_qkv(q_in, k_in, v_in);
   same_device(dout_in, q_in, "the output's gradient");
@@ -190,6 +225,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   auto delta = at::empty_like(lse);
   p.o = view_of(out);
+  if (has(lo)) p.lo = view_of(*lo);
   p.dout = view_of(dout);
   p.dq = view_of(dq);
   p.dk = view_of(dk);
@@ -336,8 +372,10 @@ void register_attention_bindings(pybind11::module_& m) {
   m.def("attention_forward", &attention_forward, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"),
         py::arg("slopes"), py::arg("causal"), py::arg("scale"), py::arg("cap"), py::arg("want_lse"));
   m.def("attention_backward", &attention_backward, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("out"), py::arg("lse"), py::arg("plan"), py::arg("slopes"), py::arg("causal"), py::arg("scale"),
+        py::arg("out"), py::arg("lse"), py::arg("lo"), py::arg("plan"), py::arg("slopes"), py::arg("causal"), py::arg("scale"),
         py::arg("cap"));
+  m.def("attention_status", [](bool reset) { return launch::attention_status(reset); }, py::arg("reset") = false,
+        "1 once a wait of a tensor-core attention kernel on the current device ran out, else 0 (waits for the device).");
   m.def("rotary_forward", &rotary_forward, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
         py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
   m.def("rotary_backward", &rotary_backward, py::arg("gq"), py::arg("gk"), py::arg("q"), py::arg("k"), py::arg("freq"),

@@ -27,6 +27,7 @@ SOURCES = [
     "csrc/kernels/noalloc_allreduce.cu",
     "csrc/kernels/attention_mask.cu",
     "csrc/kernels/attention_simt.cu",
+    "csrc/kernels/attention_tc_fwd.cu",
     "csrc/kernels/qk_norm_rotary.cu",
 ]
 

@@ -11,6 +11,8 @@ once at the end; everything else is fp32.  With P = p, A = P |v|:
   dq:  u |dq| + scale E |k|;   dk: u |dk| + scale E^T |q|
 
 where e bounds the relative error that fp32 arithmetic leaves in p and in the sums.
+float16 has a smallest step of 2^-24: p (held as 2^10 p / max p at least 2^-4) and ds also
+move by half of it, which adds 2^-31 sum|v| to o, 2^-25 to p in dv and to ds.
 """
 
 import math
@@ -85,7 +87,10 @@ def reference(q, k, v, do, *, seen, softcap=None, slopes=None, scale=None):
     E = u * ds.abs() + p * f.abs() * (u * ado + e * (dp.abs() + ado)) + e * ds.abs()
     vals = {"out": o.reshape(b, h, sq, d), "dq": dq.reshape(b, h, sq, d), "dk": dk, "dv": dv}
     tiny = torch.finfo(q.dtype).tiny  # results below it lose relative precision
-    padv = p.transpose(-1, -2) @ dod.abs()
+    step = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    E = E + step * (p > 0)
+    A = A + step / 64 * ((p > 0).double() @ vd.abs()) / (u + e)
+    padv = (p + step * (p > 0) / (u + e)).transpose(-1, -2) @ dod.abs()
     bounds = {
         "out": (u * o.abs() + (u + e) * A).reshape(b, h, sq, d) + tiny,
         "dq": (u * dq.abs() + scale * (E @ kd.abs())).reshape(b, h, sq, d) + tiny,
