@@ -23,20 +23,20 @@ constexpr int kAttnTile = 128;
 
 // The parts of a mask plan inside one int32 buffer (every part 16-byte aligned).
 struct PlanView {
-  int2* range;   // [B][Sq]   visible keys [lo, hi) of each row; (0, 0) sees none
+  int2* range;   // [B][nq * 128] visible keys [lo, hi) of each row; (0, 0) sees none, like the rows past the end
   int4* tile;    // [B][nq]   of a tile's rows: min lo, max hi of those that see a key; max lo, min hi of all
   uint4* qdead;  // [B][nq]   bit r: row r of the tile sees no key
   uint4* kdead;  // [B][nk]   bit r: key r of the tile is padding (seen by no row)
   __host__ __device__ static int64_t words(int64_t b, int64_t sq, int64_t sk) {
     const int64_t nq = (sq + kAttnTile - 1) / kAttnTile, nk = (sk + kAttnTile - 1) / kAttnTile;
-    return ((b * sq * 2 + 3) & ~int64_t(3)) + b * nq * 8 + b * nk * 4;
+    return b * nq * kAttnTile * 2 + b * nq * 8 + b * nk * 4;
   }
   __host__ __device__ static PlanView of(int* base, int64_t b, int64_t sq, int64_t sk) {
     PlanView v{nullptr, nullptr, nullptr, nullptr};
     if (base == nullptr) return v;
     const int64_t nq = (sq + kAttnTile - 1) / kAttnTile;
     v.range = reinterpret_cast<int2*>(base);
-    int* p = base + ((b * sq * 2 + 3) & ~int64_t(3));
+    int* p = base + b * nq * kAttnTile * 2;
     v.tile = reinterpret_cast<int4*>(p);
     v.qdead = reinterpret_cast<uint4*>(p + b * nq * 4);
     v.kdead = reinterpret_cast<uint4*>(p + b * nq * 8);
@@ -53,7 +53,8 @@ struct AttnParams {
   AttnTensor q, k, v, o, dout, dq, dk, dv;
   AttnTensor lo;  // o minus its rounding to the tensors' type, laid out like o (null: not kept)
   float* lse;    // [B][Hq][Sq] log2 of the softmax denominator, +inf for a row without keys
-  float* delta;  // [B][Hq][Sq] sum_d dout * o (backward)
+  float* delta;  // [B][Hq][Sq] sum_d dout * o (backward, elementary form)
+  float* stats;  // [B][Hq][nq][2][128] minus log2 of the denominator (-inf without keys, and past the end), delta
   const float* slopes;  // [Hq] or null
   PlanView plan;        // null pointers: causal or full from the lengths alone
   int b, hq, hk, sq, sk, d;
@@ -83,6 +84,8 @@ void attention_simt_backward(const AttnParams& p, cudaStream_t s);
 // allocates part_o / part_lse when there are several.
 void attention_tc_splits(const AttnParams& p, int sms, int* splits, int* split_tiles);
 cudaError_t attention_tc_forward(const AttnParams& p, cudaStream_t s);
+
+cudaError_t attention_tc_backward(const AttnParams& p, cudaStream_t s);
 
 // 0, or 1 once a wait of a tensor-core kernel on the current device ran out (its
 // outputs are NaN then); `reset` clears it.  Waits for the device.

@@ -12,7 +12,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // The keys that row i of batch entry b sees.
 __device__ __forceinline__ int2 attn_row_range(const AttnParams& p, int b, int i) {
-  if (p.plan.range != nullptr) return p.plan.range[static_cast<int64_t>(b) * p.sq + i];
+  if (p.plan.range != nullptr) return p.plan.range[static_cast<int64_t>(b) * ((p.sq + kAttnTile - 1) / kAttnTile * kAttnTile) + i];
   if (!p.causal) return make_int2(0, p.sk);
   return make_int2(0, max(0, i + p.sk - p.sq + 1));
 }
@@ -26,6 +26,16 @@ __device__ __forceinline__ int4 attn_tile_range(const AttnParams& p, int b, int 
   if (!p.causal) return make_int4(0, p.sk, 0, p.sk);
   const int first = t * kAttnTile, last = min(first + kAttnTile, p.sq) - 1;
   return make_int4(0, max(0, last + p.sk - p.sq + 1), 0, max(0, first + p.sk - p.sq + 1));
+}
+
+// Bit r: row r of row tile t sees no key.
+__device__ __forceinline__ uint4 attn_tile_qdead(const AttnParams& p, int b, int t) {
+  if (p.plan.qdead != nullptr) return p.plan.qdead[static_cast<int64_t>(b) * ((p.sq + kAttnTile - 1) / kAttnTile) + t];
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  const int none = p.causal ? p.sq - p.sk - t * kAttnTile : 0;  // rows before the first key
+  if (none > 0)
+    for (int i = 0; i < 4; ++i) w[i] = none >= 32 * (i + 1) ? 0xffffffffu : (none > 32 * i ? (1u << (none - 32 * i)) - 1u : 0u);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Whether row i sees no key, and whether key j is padding that no row sees.

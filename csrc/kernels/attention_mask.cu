@@ -114,8 +114,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const void* ids_base, in
         hi = causal ? max(pos + 1, plen) : sk;
       }
       if (hi <= lo) lo = hi = 0;
-      plan.range[static_cast<int64_t>(b) * sq + t * kAttnTile + tid] = make_int2(lo, hi);
     }
+    plan.range[(static_cast<int64_t>(b) * nq + t) * kAttnTile + tid] = make_int2(lo, hi);
     const bool some = hi > lo;
     const uint32_t dead = __ballot_sync(0xffffffffu, tid < rows && !some);
     const int w = tid >> 5;

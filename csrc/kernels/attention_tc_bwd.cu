@@ -1,0 +1,757 @@
+// Masked attention backward on the 5th-generation tensor cores.
+//
+//   stats:  -log2 sum and delta = dout.(o + what its rounding took), for both kernels below
+//   dq:     a CTA holds 128 rows of Q and dO and walks over their keys:
+//             S = Q K^T, dP = dO V^T, dS = P (dP - delta), dQ += dS K
+//   dk, dv: a CTA holds 128 keys and values and walks over the rows that see them, through all
+//           query heads that share the key head:
+//             S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//
+// Both recompute P from the saved log-sum.  Every gradient element has one owner
+// that adds in a fixed order: no atomics, the same bits every time, shared heads
+// summed in fp32.  That costs S and dP twice, seven products in place of five.
+//
+// All accumulators live in TMEM (512 columns, one CTA an SM).  P and dS go back
+// to TMEM as 16-bit values and are the TMEM operand of the second products; Q, dO
+// and K lie in shared memory once and are read along their columns by the first
+// products and along their rows by the second ones.
+//
+//   warps 0-7  arithmetic: thread = one lane of TMEM, half the 128 columns
+//   warp 8     copies, warp 9 MMAs
+//
+// The MMAs of the next tile's S and dP are issued as soon as the arithmetic has read
+// (or, where P and dS share their columns, the second product has read) the present
+// ones, so that exponentials and products run side by side.
+#include <cuda_runtime.h>
+
+#include "attention_tc.cuh"
+#include "attention_tc_host.h"
+
+namespace bitscom_b200 {
+namespace {
+
+constexpr int kCompute = 256;
+constexpr int kThreads = kCompute + 64;
+constexpr int kHalf = kAttnTile / 2;
+
+struct BwdParams {
+  AttnParams a;
+  int nq, nk;
+  int* status;
+};
+
+template <typename T>
+constexpr float prob_unshift() { return std::is_same<T, __half>::value ? 0.0009765625f : 1.f; }
+
+template <int D>
+struct Shape {
+  static constexpr int kTileBytes = kAttnTile * D * 2;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kRowBytes = 2048;  // per stage: statistics and intervals of 128 rows
+  static constexpr int kSmem = kTileBytes * (2 + 2 * kStages) + kRowBytes * kStages + 1024;
+};
+
+struct Barriers {
+  uint64_t fixed_full, s_full, s_free, p_full, dp_full, ds_full, first_done, second_done, drain;
+  uint64_t full[3], empty[3];
+};
+
+__device__ __forceinline__ void init_barriers(Barriers& bar) {
+  mbar_init(&bar.fixed_full, 1);
+  mbar_init(&bar.s_full, 1);
+  mbar_init(&bar.s_free, kCompute);
+  mbar_init(&bar.p_full, kCompute);
+  mbar_init(&bar.dp_full, 1);
+  mbar_init(&bar.ds_full, kCompute);
+  mbar_init(&bar.first_done, 1);
+  mbar_init(&bar.second_done, 1);
+  mbar_init(&bar.drain, 1);
+  for (int i = 0; i < 3; ++i) {
+    mbar_init(&bar.full[i], 1);
+    mbar_init(&bar.empty[i], 1);
+  }
+  mbar_init_fence();
+}
+
+// One product of a tile along its columns: 128 x 128 scores, contraction over D.
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t desc) {
+  for (int k = 0; k < D / 16; ++k) {
+    const uint32_t off = (k / 4) * kAttnTile * 128 + (k % 4) * 32;
+    mma_ss(d, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), desc, k > 0);
+  }
+}
+// One product with a TMEM operand: 128 x D, contraction over the 128 rows of b.  The operand's two halves, written by
+// different warps, start HALF columns apart.
+template <int HALF>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
+  for (int k = 0; k < kAttnTile / 16; ++k)
+    mma_ts(d, a + (k / 4) * HALF + (k % 4) * 8, smem_desc(b + k * 2048, kAttnTile * 128, 1024), desc, add || k > 0);
+}
+
+// Writes `cols` fp32 columns of TMEM as T, times f: one row of a [.., D] tensor.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_tmem_row(uint32_t addr, T* dst, int col0, int d, float f, bool valid, bool some,
+                                               bool ok) {
+#pragma unroll
+  for (int c = 0; c < COLS / 32; ++c) {
+    float o[32];
+    if (some && ok) {
+      tmem_ld32(addr + c * 32, reinterpret_cast<uint32_t*>(o));
+      tmem_wait_ld();
+    }
+    if (!valid) continue;
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      if (col0 + c * 32 + e >= d) continue;
+      uint4 w;
+      uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x = !ok ? __int_as_float(0x7fc00000) : (some ? o[e + 2 * k] * f : 0.f);
+        const float y = !ok ? __int_as_float(0x7fc00000) : (some ? o[e + 2 * k + 1] * f : 0.f);
+        wp[k] = pack2<T>(x, y);
+      }
+      *reinterpret_cast<uint4*>(dst + col0 + c * 32 + e) = w;
+    }
+  }
+}
+
+// --- row statistics ---------------------------------------------------------------------------------------------
+
+// LANES lanes a row, 16 bytes each.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) stats_kernel(const BwdParams bp) {
+  const AttnParams& p = bp.a;
+  constexpr int kRowsPerBlock = 256 / LANES;
+  const int64_t padded = static_cast<int64_t>(bp.nq) * kAttnTile;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / LANES;
+  if (row >= padded * p.b * p.hq) return;  // whole lane groups: padded is a multiple of them
+  const int i = static_cast<int>(row % padded);
+  const int h = static_cast<int>(row / padded % p.hq), b = static_cast<int>(row / padded / p.hq);
+  const int col = threadIdx.x % LANES * 8;
+  float sum = 0.f, lse = INFINITY;
+  if (i < p.sq) {
+    lse = p.lse[(static_cast<int64_t>(b) * p.hq + h) * p.sq + i];
+    if (col < p.d) {
+      const int64_t at = b * p.o.sb + h * p.o.sh + i * p.o.ss + col;
+      const uint4 uo = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.o.ptr) + at);
+      const uint4 ul = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo.ptr) + at);
+      const uint4 ug = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + b * p.dout.sb +
+                                                       h * p.dout.sh + i * p.dout.ss + col);
+      const T *o = reinterpret_cast<const T*>(&uo), *l = reinterpret_cast<const T*>(&ul), *g = reinterpret_cast<const T*>(&ug);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += (to_f32<T>(o[e]) + to_f32<T>(l[e])) * to_f32<T>(g[e]);
+    }
+  }
+#pragma unroll
+  for (int x = LANES / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  if (threadIdx.x % LANES == 0) {
+    float* s = p.stats + (row / kAttnTile) * 2 * kAttnTile + row % kAttnTile;
+    s[0] = -lse;
+    s[kAttnTile] = lse == INFINITY ? 0.f : sum;  // a row without keys: whatever its gradient holds
+  }
+}
+
+// --- dq ---------------------------------------------------------------------------------------------------------
+
+// Base-2 score of a raw one, and the cap's factor on its gradient.
+template <bool GENERAL>
+__device__ __forceinline__ float base2_score(float s, const ScoreScale& sc, bool capped, bool biased, float dist, float* f) {
+  if (!GENERAL) return s * sc.c;
+  float x;
+  if (capped) {
+    const float t = tanh_ex2(s * sc.cap_in);
+    x = t * sc.cap_out;
+    *f = fmaf(-t, t, 1.f);
+  } else {
+    x = s * sc.c;
+    *f = 1.f;
+  }
+  if (biased) x = fmaf(-sc.slope, fabsf(dist), x);
+  return x;
+}
+
+template <typename T, int D, bool GENERAL>
+__global__ void __launch_bounds__(kThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+              const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+              const __grid_constant__ BwdParams bp) {
+  using S = Shape<D>;
+  constexpr int kColS = 0, kColDP = 128, kColDQ = 256, kColDS = 384;  // dS: 64 columns of its own
+  const AttnParams& p = bp.a;
+  extern __shared__ char smem_raw[];
+  __shared__ Barriers bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int raised;
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* sq = base;
+  char* sdo = base + S::kTileBytes;
+  char* skv = base + 2 * S::kTileBytes;  // stages of K, V
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int id = blockIdx.x;
+  const int h = id % p.hq;
+  id /= p.hq;
+  const int b = id % p.b;
+  const int qt = bp.nq - 1 - id / p.b;  // the last rows of a causal mask see the most keys
+  const int kv_head = h / (p.hq / p.hk);
+  const int4 tr = attn_tile_range(p, b, qt);
+  const int t0 = tr.x / kAttnTile, n = max(0, (tr.y + kAttnTile - 1) / kAttnTile - t0);
+
+  if (warp == 9) {
+    tmem_alloc(&tmem_slot, 512);
+  } else if (threadIdx.x == kCompute) {
+    prefetch_tensor_map(&map_q);
+    prefetch_tensor_map(&map_do);
+    prefetch_tensor_map(&map_k);
+    prefetch_tensor_map(&map_v);
+    raised = 0;
+    init_barriers(bar);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const Guard guard{&raised, bp.status};
+
+  if (warp == 8) {
+    if (n > 0 && elect_one()) {
+      mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_4d(sq + c * kAttnTile * 128, &map_q, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
+        tma_load_4d(sdo + c * kAttnTile * 128, &map_do, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
+      }
+      int j = 0;
+      for (; j < n; ++j) {
+        const int st = j % S::kStages, ph = (j / S::kStages) & 1;
+        if (!guard.wait(&bar.empty[st], ph ^ 1)) break;
+        char* dst = skv + st * 2 * S::kTileBytes;
+        mbar_arrive_expect_tx(&bar.full[st], 2 * S::kTileBytes);
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(dst + c * kAttnTile * 128, &map_k, &bar.full[st], c * 64, (t0 + j) * kAttnTile, kv_head, b);
+          tma_load_4d(dst + S::kTileBytes + c * kAttnTile * 128, &map_v, &bar.full[st], c * 64, (t0 + j) * kAttnTile,
+                      kv_head, b);
+        }
+      }
+      if (raised) {  // no copy may be in flight when the block leaves
+        Guard::drain(&bar.fixed_full, 0);
+        for (int i = max(0, j - S::kStages); i < j; ++i) Guard::drain(&bar.full[i % S::kStages], (i / S::kStages) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (n > 0) {
+      constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
+      constexpr uint32_t kRows = mma_desc<T>(128, D, false, true);
+      const uint32_t aq = smem_addr(sq), ado = smem_addr(sdo), akv = smem_addr(skv);
+      const uint4* dead = p.plan.kdead != nullptr ? p.plan.kdead + static_cast<int64_t>(b) * bp.nk + t0 : nullptr;
+      const bool leader = elect_one();
+      bool ok = guard.wait_warp(&bar.fixed_full, 0);
+      auto stage = [&](int j) { return akv + (j % S::kStages) * 2 * S::kTileBytes; };
+      auto arrived = [&](int j) {  // K and V of tile j; padding keys cleared
+        ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
+        if (!ok) return;
+        if (dead != nullptr) {
+          const uint4 w = dead[j];
+          if (any_bit(w)) {
+            zero_dead_rows(skv + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), w, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+      };
+      auto scores = [&](int j) {
+        if (leader) {
+          mma_scores<D>(tmem + kColS, aq, stage(j), kScores);
+          mma_commit(&bar.s_full);
+        }
+        __syncwarp();
+      };
+      auto products = [&](int j) {
+        if (leader) {
+          mma_scores<D>(tmem + kColDP, ado, stage(j) + S::kTileBytes, kScores);
+          mma_commit(&bar.dp_full);
+        }
+        __syncwarp();
+      };
+      arrived(0);
+      if (ok) {
+        scores(0);
+        products(0);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) {
+          if (!(ok = guard.wait_warp(&bar.s_free, j & 1))) break;
+          arrived(j + 1);
+          if (!ok) break;
+          tc_fence_after();
+          scores(j + 1);
+        }
+        if (!(ok = guard.wait_warp(&bar.ds_full, j & 1))) break;
+        tc_fence_after();
+        if (j + 1 < n) products(j + 1);
+        if (leader) {
+          mma_rows<32>(tmem + kColDQ, tmem + kColDS, stage(j), kRows, j > 0);
+          mma_commit(&bar.empty[j % S::kStages]);
+          mma_commit(&bar.second_done);
+        }
+        __syncwarp();
+      }
+      if (!ok) {  // no MMA may be in flight when TMEM is freed
+        if (leader) {
+          mma_commit(&bar.drain);
+          Guard::drain(&bar.drain, 0);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int r = (warp % 4) * 32 + lane, half = warp / 4;
+    const int i = qt * kAttnTile + r;
+    const bool valid = i < p.sq;
+    const int2 range = valid ? attn_row_range(p, b, i) : make_int2(0, 0);
+    const int pos = i + p.sk - p.sq;
+    const ScoreScale sc = ScoreScale::of(p, h);
+    const float* st = p.stats + ((static_cast<int64_t>(b) * p.hq + h) * bp.nq + qt) * 2 * kAttnTile + r;
+    const float nlse = st[0] + prob_shift<T>(), delta = st[kAttnTile];
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int key0 = (t0 + j) * kAttnTile + half * kHalf;
+      const bool full = tr.z <= key0 && tr.w >= key0 + kHalf;
+      if (!(ok = guard.wait_warp(&bar.s_full, j & 1))) break;
+      tc_fence_after();
+      float pf[kHalf];  // probability times the cap's factor
+      tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
+      tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive(&bar.s_free);
+      const float d0 = static_cast<float>(key0 - pos);
+#pragma unroll
+      for (int c = 0; c < kHalf; ++c) {
+        float f = 1.f;
+        if (GENERAL) {
+          const float x = base2_score<GENERAL>(pf[c], sc, p.cap > 0.f, p.slopes != nullptr, d0 + c, &f);
+          pf[c] = ex2(x + nlse) * (prob_unshift<T>() * f);
+        } else {
+          pf[c] = ex2(fmaf(pf[c], sc.c, nlse));
+          if (prob_unshift<T>() != 1.f) pf[c] *= prob_unshift<T>();
+        }
+      }
+      if (!full) {
+        const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
+#pragma unroll
+        for (int c = 0; c < kHalf; ++c) pf[c] = from + c < len ? pf[c] : 0.f;
+      }
+      if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float dp[32];
+        tmem_ld32(lanes + kColDP + half * kHalf + c * 32, reinterpret_cast<uint32_t*>(dp));
+        tmem_wait_ld();
+        if (full) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            w[c * 16 + e / 2] = pack2<T>(pf[c * 32 + e] * (dp[e] - delta), pf[c * 32 + e + 1] * (dp[e + 1] - delta));
+        } else {  // a masked pair is zero, whatever its product is
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float x = pf[c * 32 + e], y = pf[c * 32 + e + 1];
+            w[c * 16 + e / 2] = pack2<T>(x == 0.f ? 0.f : x * (dp[e] - delta), y == 0.f ? 0.f : y * (dp[e + 1] - delta));
+          }
+        }
+      }
+      if (j > 0) {  // the last dS has been read
+        if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
+        tc_fence_after();
+      }
+      tmem_st32(lanes + kColDS + half * 32, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.ds_full);
+    }
+    if (ok && n > 0) {
+      ok = guard.wait_warp(&bar.second_done, (n - 1) & 1);
+      tc_fence_after();
+    }
+    T* dst = static_cast<T*>(p.dq.ptr) + b * p.dq.sb + h * p.dq.sh + i * p.dq.ss;
+    store_tmem_row<T, D / 2>(lanes + kColDQ + half * (D / 2), dst, half * (D / 2), p.d, p.scale, valid, n > 0, ok);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+// --- dk, dv -----------------------------------------------------------------------------------------------------
+
+// The (query head, row tile) pairs that see a tile of keys, in order.
+struct RowTiles {
+  const AttnParams* p;
+  int b, key0, first, last, group;
+  int g, t;
+  bool full;  // every row of the tile sees every key
+  __device__ bool take() {
+    const int4 r = attn_tile_range(*p, b, t);
+    full = r.z <= key0 && r.w >= key0 + kAttnTile;
+    return r.y > key0 && r.x < key0 + kAttnTile;
+  }
+  __device__ bool begin() {
+    g = 0;
+    t = first;
+    if (first > last) return false;
+    return take() || next();
+  }
+  __device__ bool next() {
+    for (;;) {
+      if (++t > last) {
+        t = first;
+        if (++g == group) return false;
+      }
+      if (take()) return true;
+    }
+  }
+};
+
+template <typename T, int D, bool GENERAL>
+__global__ void __launch_bounds__(kThreads, 1)
+    dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+               const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+               const __grid_constant__ BwdParams bp) {
+  using S = Shape<D>;
+  // D = 64 leaves room for P and dS beside S and dP; else each half of the warps writes
+  // them over the scores that it alone has read.
+  constexpr bool kOwn = D == 64;
+  constexpr int kHalfCols = kOwn ? 32 : 64;
+  constexpr int kColS = 0, kColDP = 128, kColDV = 256, kColDK = 256 + D;
+  constexpr int kColP = kOwn ? 384 : kColS, kColDS = kOwn ? 448 : kColDP;
+  const AttnParams& p = bp.a;
+  extern __shared__ char smem_raw[];
+  __shared__ Barriers bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int raised, first_tile, last_tile;
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* sk = base;
+  char* sv = base + S::kTileBytes;
+  char* sqd = base + 2 * S::kTileBytes;  // stages of Q, dO
+  char* rows = sqd + S::kStages * 2 * S::kTileBytes;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int id = blockIdx.x;
+  const int hk = id % p.hk;
+  id /= p.hk;
+  const int b = id % p.b;
+  const int key0 = id / p.b * kAttnTile;  // the first keys of a causal mask are seen by the most rows
+  const int group = p.hq / p.hk;
+
+  if (warp == 9) {
+    tmem_alloc(&tmem_slot, 512);
+  } else if (threadIdx.x == kCompute) {
+    prefetch_tensor_map(&map_q);
+    prefetch_tensor_map(&map_do);
+    prefetch_tensor_map(&map_k);
+    prefetch_tensor_map(&map_v);
+    raised = 0;
+    first_tile = 0x7fffffff;
+    last_tile = -1;
+    init_barriers(bar);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  {  // the first and last row tile that see a key of this tile
+    int a = 0x7fffffff, z = -1;
+    for (int t = threadIdx.x; t < bp.nq; t += kThreads) {
+      const int4 r = attn_tile_range(p, b, t);
+      if (r.y > key0 && r.x < key0 + kAttnTile) {
+        a = min(a, t);
+        z = t;
+      }
+    }
+    a = __reduce_min_sync(0xffffffffu, a);
+    z = __reduce_max_sync(0xffffffffu, z);
+    if (lane == 0 && z >= 0) {
+      atomicMin(&first_tile, a);
+      atomicMax(&last_tile, z);
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = tmem_slot;
+  const Guard guard{&raised, bp.status};
+  RowTiles it{&p, b, key0, first_tile, last_tile, group, 0, 0, false};
+  const bool some = it.begin();
+
+  if (warp == 8) {
+    if (some && elect_one()) {
+      mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_4d(sk + c * kAttnTile * 128, &map_k, &bar.fixed_full, c * 64, key0, hk, b);
+        tma_load_4d(sv + c * kAttnTile * 128, &map_v, &bar.fixed_full, c * 64, key0, hk, b);
+      }
+      int j = 0;
+      bool more = true;
+      for (; more; ++j, more = it.next()) {
+        const int st = j % S::kStages, ph = (j / S::kStages) & 1;
+        if (!guard.wait(&bar.empty[st], ph ^ 1)) break;
+        const int h = hk * group + it.g;
+        char* dst = sqd + st * 2 * S::kTileBytes;
+        char* rd = rows + st * S::kRowBytes;
+        mbar_arrive_expect_tx(&bar.full[st], 2 * S::kTileBytes + (p.plan.range != nullptr ? 2048 : 1024));
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(dst + c * kAttnTile * 128, &map_q, &bar.full[st], c * 64, it.t * kAttnTile, h, b);
+          tma_load_4d(dst + S::kTileBytes + c * kAttnTile * 128, &map_do, &bar.full[st], c * 64, it.t * kAttnTile, h, b);
+        }
+        bulk_g2s(rd, p.stats + ((static_cast<int64_t>(b) * p.hq + h) * bp.nq + it.t) * 2 * kAttnTile, 1024, &bar.full[st]);
+        if (p.plan.range != nullptr)
+          bulk_g2s(rd + 1024, p.plan.range + (static_cast<int64_t>(b) * bp.nq + it.t) * kAttnTile, 1024, &bar.full[st]);
+      }
+      if (raised) {  // no copy may be in flight when the block leaves
+        Guard::drain(&bar.fixed_full, 0);
+        for (int i = max(0, j - S::kStages); i < j; ++i) Guard::drain(&bar.full[i % S::kStages], (i / S::kStages) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (some) {
+      constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
+      constexpr uint32_t kRows = mma_desc<T>(128, D, false, true);
+      const uint32_t ak = smem_addr(sk), av = smem_addr(sv), aqd = smem_addr(sqd);
+      const bool leader = elect_one();
+      bool ok = guard.wait_warp(&bar.fixed_full, 0);
+      auto stage = [&](int j) { return aqd + (j % S::kStages) * 2 * S::kTileBytes; };
+      auto arrived = [&](int j) {  // Q and dO of step j; rows without keys cleared
+        ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
+        if (!ok || it.full) return;
+        const uint4 w = attn_tile_qdead(p, b, it.t);
+        if (any_bit(w)) {
+          zero_dead_rows(sqd + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), w, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      };
+      auto scores = [&](int j) {
+        if (leader) {
+          mma_scores<D>(tmem + kColS, ak, stage(j), kScores);
+          mma_commit(&bar.s_full);
+        }
+        __syncwarp();
+      };
+      auto products = [&](int j) {
+        if (leader) {
+          mma_scores<D>(tmem + kColDP, av, stage(j) + S::kTileBytes, kScores);
+          mma_commit(&bar.dp_full);
+        }
+        __syncwarp();
+      };
+      auto add_dv = [&](int j) {
+        if (leader) {
+          mma_rows<kHalfCols>(tmem + kColDV, tmem + kColP, stage(j) + S::kTileBytes, kRows, j > 0);
+          mma_commit(&bar.first_done);
+        }
+        __syncwarp();
+      };
+      auto add_dk = [&](int j) {
+        if (leader) {
+          mma_rows<kHalfCols>(tmem + kColDK, tmem + kColDS, stage(j), kRows, j > 0);
+          mma_commit(&bar.empty[j % S::kStages]);
+          mma_commit(&bar.second_done);
+        }
+        __syncwarp();
+      };
+      arrived(0);
+      if (ok) {
+        scores(0);
+        products(0);
+      }
+      bool more = ok;
+      for (int j = 0; more && ok; ++j) {
+        more = it.next();
+        if (!(ok = guard.wait_warp(&bar.p_full, j & 1))) break;
+        tc_fence_after();
+        if (kOwn) {
+          if (more) {
+            arrived(j + 1);
+            if (!ok) break;
+            scores(j + 1);
+          }
+          add_dv(j);
+        } else {
+          add_dv(j);
+          if (more) {
+            arrived(j + 1);
+            if (!(ok = ok && guard.wait_warp(&bar.first_done, j & 1))) break;
+            scores(j + 1);
+          }
+        }
+        if (!(ok = guard.wait_warp(&bar.ds_full, j & 1))) break;
+        tc_fence_after();
+        if (kOwn) {
+          if (more) products(j + 1);
+          add_dk(j);
+        } else {
+          add_dk(j);
+          if (more) {
+            if (!(ok = guard.wait_warp(&bar.second_done, j & 1))) break;
+            products(j + 1);
+          }
+        }
+      }
+      if (!ok) {  // no MMA may be in flight when TMEM is freed
+        if (leader) {
+          mma_commit(&bar.drain);
+          Guard::drain(&bar.drain, 0);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int r = (warp % 4) * 32 + lane, half = warp / 4;
+    const int key = key0 + r;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
+    bool ok = true, more = some;
+    int j = 0;
+    for (; more; ++j) {
+      const int st = j % S::kStages;
+      const float* stats = reinterpret_cast<const float*>(rows + st * S::kRowBytes) + half * kHalf;
+      const int2* range = reinterpret_cast<const int2*>(rows + st * S::kRowBytes + 1024) + half * kHalf;
+      const int row0 = it.t * kAttnTile + half * kHalf;
+      const bool full = it.full;
+      const ScoreScale sc = ScoreScale::of(p, hk * group + it.g);
+      more = it.next();
+      if (!(ok = guard.wait_warp(&bar.full[st], (j / S::kStages) & 1) && guard.wait_warp(&bar.s_full, j & 1))) break;
+      tc_fence_after();
+      float pf[kHalf];  // probability times the cap's factor
+      tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
+      tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
+      tmem_wait_ld();
+      uint32_t w[32];
+      const float d0 = static_cast<float>(row0 + p.sk - p.sq - key);
+      unsigned seen[2] = {0xffffffffu, 0xffffffffu};  // which of the 64 rows see this key
+      if (!full && (p.causal || p.plan.range != nullptr)) {
+        seen[0] = seen[1] = 0u;
+        if (p.plan.range != nullptr) {
+#pragma unroll
+          for (int c = 0; c < kHalf; ++c) {
+            const int2 v = range[c];
+            if (key >= v.x && key < v.y) seen[c / 32] |= 1u << (c % 32);
+          }
+        } else {  // causal: rows from key - (Sk - Sq) on
+          const int from = key - (row0 + p.sk - p.sq);
+#pragma unroll
+          for (int c = 0; c < kHalf; ++c)
+            if (c >= from) seen[c / 32] |= 1u << (c % 32);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 4) {
+        const float4 nl = *reinterpret_cast<const float4*>(stats + c);
+        const float nlse[4] = {nl.x, nl.y, nl.z, nl.w};
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f = 1.f;
+          float x = base2_score<GENERAL>(pf[c + e], sc, p.cap > 0.f, p.slopes != nullptr, d0 + (c + e), &f);
+          x = GENERAL ? x + (nlse[e] + prob_shift<T>()) : fmaf(pf[c + e], sc.c, nlse[e] + prob_shift<T>());
+          pr[e] = ex2(x);
+          if (!full) pr[e] = (seen[c / 32] >> ((c + e) % 32)) & 1u ? pr[e] : 0.f;
+          pf[c + e] = GENERAL || prob_unshift<T>() != 1.f ? pr[e] * (prob_unshift<T>() * f) : pr[e];
+        }
+        w[c / 2] = pack2<T>(pr[0], pr[1]);
+        w[c / 2 + 1] = pack2<T>(pr[2], pr[3]);
+      }
+      if (kOwn && j > 0) {  // the last P has been read
+        if (!(ok = guard.wait_warp(&bar.first_done, (j - 1) & 1))) break;
+        tc_fence_after();
+      }
+      tmem_st32(lanes + kColP + half * kHalfCols, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.p_full);
+      if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float dp[32];
+        tmem_ld32(lanes + kColDP + half * kHalf + c * 32, reinterpret_cast<uint32_t*>(dp));
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 dl = *reinterpret_cast<const float4*>(stats + kAttnTile + c * 32 + e);
+          float ds[4] = {dp[e] - dl.x, dp[e + 1] - dl.y, dp[e + 2] - dl.z, dp[e + 3] - dl.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = pf[c * 32 + e + k];
+            ds[k] = !full && x == 0.f ? 0.f : x * ds[k];  // a masked pair is zero, whatever its product is
+          }
+          w[c * 16 + e / 2] = pack2<T>(ds[0], ds[1]);
+          w[c * 16 + e / 2 + 1] = pack2<T>(ds[2], ds[3]);
+        }
+      }
+      if (kOwn && j > 0) {  // the last dS has been read
+        if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
+        tc_fence_after();
+      }
+      tmem_st32(lanes + kColDS + half * kHalfCols, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.ds_full);
+    }
+    if (ok && some) {
+      ok = guard.wait_warp(&bar.second_done, (j - 1) & 1);
+      tc_fence_after();
+    }
+    const bool valid = key < p.sk;
+    const int col = half * (D / 2);
+    T* dv = static_cast<T*>(p.dv.ptr) + b * p.dv.sb + hk * p.dv.sh + key * p.dv.ss;
+    T* dk = static_cast<T*>(p.dk.ptr) + b * p.dk.sb + hk * p.dk.sh + key * p.dk.ss;
+    store_tmem_row<T, D / 2>(lanes + kColDV + col, dv, col, p.d, prob_unshift<T>(), valid, some, ok);
+    store_tmem_row<T, D / 2>(lanes + kColDK + col, dk, col, p.d, p.scale, valid, some, ok);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+template <typename T, int D, bool GENERAL>
+cudaError_t run(const BwdParams& bp, cudaStream_t s) {
+  const AttnParams& p = bp.a;
+  CUtensorMap q, g, k, v;
+  if (!attn_map(&q, p.q, p, p.hq, p.sq, kAttnTile, 1) || !attn_map(&g, p.dout, p, p.hq, p.sq, kAttnTile, 1) ||
+      !attn_map(&k, p.k, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, kAttnTile, 1))
+    return cudaErrorInvalidValue;
+  constexpr int kLanes = D / 8, kRowsPerBlock = 256 / kLanes;
+  const int64_t rows = static_cast<int64_t>(bp.nq) * kAttnTile * p.b * p.hq;
+  stats_kernel<T, kLanes><<<static_cast<unsigned>((rows + kRowsPerBlock - 1) / kRowsPerBlock), 256, 0, s>>>(bp);
+  cudaError_t e = cudaFuncSetAttribute(dq_kernel<T, D, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(dkv_kernel<T, D, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  dq_kernel<T, D, GENERAL>
+      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nq) * p.b * p.hq), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, bp);
+  dkv_kernel<T, D, GENERAL>
+      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nk) * p.b * p.hk), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, bp);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t by_scores(const BwdParams& bp, cudaStream_t s) {
+  return bp.a.cap > 0.f || bp.a.slopes != nullptr ? run<T, D, true>(bp, s) : run<T, D, false>(bp, s);
+}
+
+}  // namespace
+
+namespace launch {
+
+cudaError_t attention_tc_backward(const AttnParams& p, cudaStream_t s) {
+  BwdParams bp{p, (p.sq + kAttnTile - 1) / kAttnTile, (p.sk + kAttnTile - 1) / kAttnTile, attn_status_ptr()};
+  if (p.dt == kBF16) return p.d <= 64 ? by_scores<__nv_bfloat16, 64>(bp, s) : by_scores<__nv_bfloat16, 128>(bp, s);
+  return p.d <= 64 ? by_scores<__half, 64>(bp, s) : by_scores<__half, 128>(bp, s);
+}
+
+}  // namespace launch
+}  // namespace bitscom_b200

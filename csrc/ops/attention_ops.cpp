@@ -223,7 +223,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     return {dq, dk, dv};
   }
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
-  auto delta = at::empty_like(lse);
   p.o = view_of(out);
   if (has(lo)) p.lo = view_of(*lo);
   p.dout = view_of(dout);
@@ -231,9 +230,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
   p.dk = view_of(dk);
   p.dv = view_of(dv);
   p.lse = lse.data_ptr<float>();
-  p.delta = delta.data_ptr<float>();
-  launch::attention_simt_backward(p, stream_of(q));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (for_tensor_cores(q)) {
+    TORCH_CHECK(has(lo), "bitscom: the forward pass kept no rounding of its output");
+    const int64_t tiles = (q.size(2) + kAttnTile - 1) / kAttnTile;
+    auto stats = at::empty({q.size(0), q.size(1), tiles, 2, kAttnTile}, lse.options());
+    p.stats = stats.data_ptr<float>();
+    C10_CUDA_CHECK(launch::attention_tc_backward(p, stream_of(q)));
+  } else {
+    auto delta = at::empty_like(lse);
+    p.delta = delta.data_ptr<float>();
+    launch::attention_simt_backward(p, stream_of(q));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
   return {dq, dk, dv};
 }
 

@@ -28,6 +28,7 @@ SOURCES = [
     "csrc/kernels/attention_mask.cu",
     "csrc/kernels/attention_simt.cu",
     "csrc/kernels/attention_tc_fwd.cu",
+    "csrc/kernels/attention_tc_bwd.cu",
     "csrc/kernels/qk_norm_rotary.cu",
 ]
 

@@ -12,7 +12,9 @@ once at the end; everything else is fp32.  With P = p, A = P |v|:
 
 where e bounds the relative error that fp32 arithmetic leaves in p and in the sums.
 float16 has a smallest step of 2^-24: p (held as 2^10 p / max p at least 2^-4) and ds also
-move by half of it, which adds 2^-31 sum|v| to o, 2^-25 to p in dv and to ds.
+move by half of it, which adds 2^-31 sum|v| to o, 2^-25 to p in dv and to ds.  In every type p is
+an fp32 value, so one below 2^-126 (a score 88 under the row's log-sum) counts as zero: p moves by
+up to 2^-126, ds by 2^-126 (|dp| + sum|do||o|), and both by 2^-126 where ds or p itself is below it.
 """
 
 import math
@@ -88,9 +90,10 @@ def reference(q, k, v, do, *, seen, softcap=None, slopes=None, scale=None):
     vals = {"out": o.reshape(b, h, sq, d), "dq": dq.reshape(b, h, sq, d), "dk": dk, "dv": dv}
     tiny = torch.finfo(q.dtype).tiny  # results below it lose relative precision
     step = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
-    E = E + step * (p > 0)
-    A = A + step / 64 * ((p > 0).double() @ vd.abs()) / (u + e)
-    padv = (p + step * (p > 0) / (u + e)).transpose(-1, -2) @ dod.abs()
+    least = 2.0 ** -126
+    E = E + (step + least * (1 + dp.abs() + ado)) * (p > 0)
+    A = A + (step / 64 + least) * ((p > 0).double() @ vd.abs()) / (u + e)
+    padv = (p + (step + least) * (p > 0) / (u + e)).transpose(-1, -2) @ dod.abs()
     bounds = {
         "out": (u * o.abs() + (u + e) * A).reshape(b, h, sq, d) + tiny,
         "dq": (u * dq.abs() + scale * (E @ kd.abs())).reshape(b, h, sq, d) + tiny,
