@@ -9,6 +9,8 @@ random-init weights; AdamW.
     python -m torch.distributed.run --nproc-per-node 8 --master-addr 127.0.0.1 \
         benchmarks/gpt2_fsdp.py --steps 10 --warmup 3
     ... --comm nccl        # fp32 NCCL reduce-scatter / all-gather (baseline)
+    ... --documents 4      # rows of packed documents (document mask), with --rotary / --softcap C:
+                           # queries and keys normalised and rotated, attention scores capped
     ... --fsdp2            # PyTorch FSDP2 (fully_shard per block) on a `lowbit`
                            # process group (or on NCCL with --comm nccl)
 
@@ -44,6 +46,17 @@ from bitscom_b200.models import gpt2_medium, gpt2_small_test  # noqa: E402
 from bitscom_b200.parallel.fsdp import LowBitShardedDP  # noqa: E402
 
 
+def packed(args, rank):
+    """Document ids of the rows ([micro_batch, seq]; random lengths), or None."""
+    if args.documents <= 1:
+        return None
+    g = torch.Generator().manual_seed(77 + rank)
+    cuts = torch.randint(1, args.seq, (args.micro_batch, args.documents - 1), generator=g)
+    ids = torch.zeros(args.micro_batch, args.seq, dtype=torch.int32)
+    ids.scatter_add_(1, cuts, torch.ones_like(cuts, dtype=torch.int32))
+    return ids.cumsum(1, dtype=torch.int32).cuda()
+
+
 def main():
     p = argparse.ArgumentParser()
     p.add_argument("--steps", type=int, default=10)
@@ -59,6 +72,9 @@ def main():
                    help="low-bit FSDP2 collectives: per-module custom comms on an NCCL group (error feedback per "
                         "module) or the `lowbit` backend's fused RS/AG under FSDP2's default comms")
     p.add_argument("--no-ef", action="store_true")
+    p.add_argument("--documents", type=int, default=0, help="documents packed into every row (0: one, no mask)")
+    p.add_argument("--rotary", action="store_true", help="norm and rotation of queries and keys, no position table")
+    p.add_argument("--softcap", type=float, default=None, help="cap of the attention scores")
     args = p.parse_args()
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -79,7 +95,8 @@ def main():
     dist.init_process_group(backend, timeout=datetime.timedelta(seconds=300), device_id=torch.device("cuda", local), **kw)
 
     torch.manual_seed(0)
-    model = (gpt2_small_test() if args.small else gpt2_medium()).cuda()
+    options = dict(rotary=args.rotary, softcap=args.softcap)
+    model = (gpt2_small_test(**options) if args.small else gpt2_medium(**options)).cuda()
     if args.fsdp2:
         run_fsdp2(model, args, world, rank, lowbit)
         return
@@ -95,11 +112,12 @@ def main():
     vocab = model.cfg.vocab_size
     g = torch.Generator(device="cuda").manual_seed(1000 + rank)
     pool = [torch.randint(0, vocab, (args.micro_batch, args.seq + 1), device="cuda", generator=g) for _ in range(4)]
+    docs = packed(args, rank)
 
     def step(i):
         tok = pool[i % len(pool)]
         with torch.autocast("cuda", dtype=torch.bfloat16):
-            _, loss = sdp(tok[:, :-1], tok[:, 1:])
+            _, loss = sdp(tok[:, :-1], tok[:, 1:], documents=docs)
         loss.backward()
         sdp.step()
         return loss
@@ -129,7 +147,8 @@ def main():
             "dtype": "bf16", "data": "synthetic uniform tokens", "loss": float(loss.item()),
             "config": {"model": "gpt2_small_test" if args.small else "gpt2_medium", "micro_batch": args.micro_batch,
                        "seq_len": args.seq, "comm": f"{args.bits}-bit EF low-bit RS/AG" if lowbit else "fp32 NCCL RS/AG",
-                       "fmt": "e4m3" if args.fp8 else "int", "parallelism": f"zero3-dp{world}"},
+                       "fmt": "e4m3" if args.fp8 else "int", "documents": args.documents, "rotary": args.rotary,
+                       "softcap": args.softcap, "parallelism": f"zero3-dp{world}"},
         }), flush=True)
     dist.barrier()
     dist.destroy_process_group()
@@ -155,11 +174,12 @@ def run_fsdp2(model, args, world, rank, lowbit):
     vocab = model.cfg.vocab_size
     g = torch.Generator(device="cuda").manual_seed(1000 + rank)
     pool = [torch.randint(0, vocab, (args.micro_batch, args.seq + 1), device="cuda", generator=g) for _ in range(4)]
+    docs = packed(args, rank)
 
     def step(i):
         tok = pool[i % len(pool)]
         with torch.autocast("cuda", dtype=torch.bfloat16):
-            _, loss = model(tok[:, :-1], tok[:, 1:])
+            _, loss = model(tok[:, :-1], tok[:, 1:], documents=docs)
         loss.backward()
         opt.step()
         opt.zero_grad(set_to_none=True)
@@ -203,7 +223,8 @@ def run_fsdp2(model, args, world, rank, lowbit):
                                  ("per-module custom comms" + ("" if args.no_ef else ", EF on gradients")
                                   if comms is not None else "lowbit backend" + ("" if args.no_ef else ", EF")))
                                 if lowbit else "fp32 NCCL RS/AG"),
-                       "fmt": "e4m3" if args.fp8 else "int", "parallelism": f"fsdp2-dp{world}"},
+                       "fmt": "e4m3" if args.fp8 else "int", "documents": args.documents, "rotary": args.rotary,
+                       "softcap": args.softcap, "parallelism": f"fsdp2-dp{world}"},
         }), flush=True)
     dist.barrier()
     dist.destroy_process_group()

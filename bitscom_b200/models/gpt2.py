@@ -7,6 +7,12 @@ tied to the token embedding.  Attention uses
 used Hugging Face's GPT2LMHeadModel with a 4-layer/256-wide config (reference
 benchmarks/multimodel_stochastic_e2e_curve.py:62-74); :func:`gpt2_medium` is
 the 24-layer / 1024-wide / 16-head model of the sharded benchmark config.
+
+Options beyond GPT-2, off by default (:class:`GPT2Config`): queries and keys
+normalised for each head and rotated by position in place of the learned
+position table, capped attention scores, a distance bias; and, as arguments of
+``forward``, rows of packed documents and prefixes.  With any of them attention
+runs through :func:`bitscom_b200.ops.attention`.
 """
 
 from __future__ import annotations
@@ -18,6 +24,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.attention import attention, attention_mask
+from ..ops.rotary import qk_norm_rotary, rotary_frequencies
+
 
 @dataclass
 class GPT2Config:
@@ -27,6 +36,9 @@ class GPT2Config:
     n_layer: int = 24
     n_head: int = 16
     dropout: float = 0.0
+    rotary: bool = False  # norm of queries and keys per head + rotation, no position table
+    softcap: float | None = None  # cap of the attention scores
+    distance_bias: bool = False  # slope 2^(-8 h / n_head) times the distance off head h's scores
 
 
 class _Attention(nn.Module):
@@ -35,13 +47,36 @@ class _Attention(nn.Module):
         self.n_head = cfg.n_head
         self.qkv = nn.Linear(cfg.n_embd, 3 * cfg.n_embd)
         self.proj = nn.Linear(cfg.n_embd, cfg.n_embd)
+        self.softcap = cfg.softcap
+        self.rotary, self.distance_bias = cfg.rotary, cfg.distance_bias
+        if cfg.rotary:
+            self.q_gain = nn.Parameter(torch.ones(cfg.n_embd // cfg.n_head))
+            self.k_gain = nn.Parameter(torch.ones(cfg.n_embd // cfg.n_head))
+        # Constants, kept out of the buffers: a cast of the module must not round the float64 frequencies.
+        self._constants = {}
 
-    def forward(self, x):
+    def _constant(self, name: str, device: torch.device) -> torch.Tensor:
+        if (name, device) not in self._constants:
+            if name == "frequencies":
+                d = self.qkv.in_features // self.n_head
+                value = rotary_frequencies(d - d % 2)
+            else:
+                value = 2.0 ** (-8.0 * torch.arange(1, self.n_head + 1, dtype=torch.float32) / self.n_head)
+            self._constants[name, device] = value.to(device)
+        return self._constants[name, device]
+
+    def forward(self, x, mask=None):
         b, t, c = x.shape
-        q, k, v = self.qkv(x).split(c, dim=2)
-        shape = (b, t, self.n_head, c // self.n_head)
-        q, k, v = (z.view(shape).transpose(1, 2) for z in (q, k, v))
-        y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        q, k, v = (z.view(b, t, self.n_head, c // self.n_head) for z in self.qkv(x).split(c, dim=2))
+        if self.rotary:
+            q, k = qk_norm_rotary(q, k, self._constant("frequencies", x.device), q_weight=self.q_gain,
+                                  k_weight=self.k_gain)
+        q, k, v = (z.transpose(1, 2) for z in (q, k, v))
+        if mask is None and self.softcap is None and not self.distance_bias:
+            y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        else:
+            slopes = self._constant("slopes", x.device) if self.distance_bias else None
+            y = attention(q, k, v, mask=mask, softcap=self.softcap, slopes=slopes)
         return self.proj(y.transpose(1, 2).reshape(b, t, c))
 
 
@@ -54,8 +89,8 @@ class _Block(nn.Module):
         self.fc = nn.Linear(cfg.n_embd, 4 * cfg.n_embd)
         self.out = nn.Linear(4 * cfg.n_embd, cfg.n_embd)
 
-    def forward(self, x):
-        x = x + self.attn(self.ln1(x))
+    def forward(self, x, mask=None):
+        x = x + self.attn(self.ln1(x), mask)
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
 
@@ -64,7 +99,7 @@ class GPT2(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.wte = nn.Embedding(cfg.vocab_size, cfg.n_embd)
-        self.wpe = nn.Embedding(cfg.n_positions, cfg.n_embd)
+        self.wpe = None if cfg.rotary else nn.Embedding(cfg.n_positions, cfg.n_embd)
         self.blocks = nn.ModuleList([_Block(cfg) for _ in range(cfg.n_layer)])
         self.ln_f = nn.LayerNorm(cfg.n_embd)
         self.apply(self._init)
@@ -81,12 +116,31 @@ class GPT2(nn.Module):
         elif isinstance(m, nn.Embedding):
             nn.init.normal_(m.weight, 0.0, 0.02)
 
-    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
+    def forward(
+        self,
+        idx: torch.Tensor,
+        targets: torch.Tensor | None = None,
+        documents: torch.Tensor | None = None,
+        prefix: torch.Tensor | None = None,
+    ):
+        """Logits, or ``(logits, mean loss)`` with targets (-100: not counted).
+
+        ``documents`` [batch, length]: ids of documents packed into the rows
+        (tokens see their own one, positions restart with each; negative:
+        padding).  ``prefix`` [batch]: leading tokens that all see each other.
+        """
         t = idx.shape[1]
-        pos = torch.arange(t, device=idx.device)
-        x = self.wte(idx) + self.wpe(pos)
+        mask = None if documents is None and prefix is None else attention_mask(documents, prefix, q_len=t, k_len=t)
+        x = self.wte(idx)
+        if self.wpe is not None:
+            pos = torch.arange(t, device=idx.device)
+            if documents is not None:
+                starts = torch.ones_like(documents, dtype=torch.bool)
+                starts[:, 1:] = documents[:, 1:] != documents[:, :-1]
+                pos = pos - torch.where(starts, pos, 0).cummax(dim=1).values
+            x = x + self.wpe(pos)
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x, mask)
         logits = F.linear(self.ln_f(x), self.wte.weight)
         if targets is None:
             return logits
