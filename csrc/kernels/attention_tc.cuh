@@ -15,29 +15,129 @@ constexpr float prob_shift() { return std::is_same<T, __half>::value ? 10.f : 0.
 // and right at both ends (e^2x = inf, 0).
 __device__ __forceinline__ float tanh_ex2(float x2log2e) { return fmaf(-2.f, rcp(1.f + ex2(x2log2e)), 1.f); }
 
-// Score constants of a launch and head.
+// Near zero tanh(x) = x P(x^2), coefficients fitted (least squares, reweighted towards the
+// largest error): three on |x| <= 0.3 to an absolute error of 1.7e-7, five on |x| <= 0.6 to 3e-8.
+constexpr float kTanhNear = 0.3f, kTanhMid = 0.6f;
+constexpr float kTanhPoly3[3] = {0.99999601f, -0.33297479f, 0.1252259f};
+constexpr float kTanhPoly5[5] = {0.99999964f, -0.33331209f, 0.13299210f, -0.05169674f, 0.014976959f};
+
+// Score constants of a launch, computed on the host: operands from the constant bank.
 struct ScoreScale {
-  float c;       // plain: scale * log2 e
-  float cap_in;  // capped: 2 log2 e * scale / cap
-  float cap_out; // capped: cap * log2 e
-  float slope;   // distance: slope * log2 e
-  __device__ static ScoreScale of(const AttnParams& p, int h) {
-    ScoreScale s;
+  float c;        // plain: scale * log2 e
+  float cap_in;   // capped: 2 log2 e * scale / cap
+  float cap_out;  // capped: cap * log2 e
+  float cap_inv;  // capped: 1 / cap_out
+  float near, mid;          // capped: largest raw scores of the polynomials
+  float poly3[3], poly5[5];  // capped: the polynomials for raw scores, times cap_out
+  static ScoreScale of(const AttnParams& p) {
+    ScoreScale s{};
     s.c = p.scale * kLog2e;
-    s.cap_in = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f;
-    s.cap_out = p.cap * kLog2e;
-    s.slope = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+    if (p.cap > 0.f) {
+      const float k = p.scale / p.cap;
+      s.cap_out = p.cap * kLog2e;
+      s.cap_in = 2.f * kLog2e * k;
+      s.cap_inv = 1.f / s.cap_out;
+      s.near = kTanhNear / k;
+      s.mid = kTanhMid / k;
+      float f = k * s.cap_out;
+      for (int i = 0; i < 5; ++i, f *= k * k) {
+        if (i < 3) s.poly3[i] = kTanhPoly3[i] * f;
+        s.poly5[i] = kTanhPoly5[i] * f;
+      }
+    }
     return s;
   }
 };
 
-// One 128 x 128 (or narrower) operand tile: sub-tiles of 64 columns.
-__device__ __forceinline__ void zero_dead_rows(char* tile, int subtiles, const uint4& dead, int lane) {
-  const uint32_t w[4] = {dead.x, dead.y, dead.z, dead.w};
-  for (int r = 0; r < kAttnTile; ++r) {
-    if (!((w[r >> 5] >> (r & 31)) & 1u)) continue;
+// What a launch does to its scores; kCapped covers capped scores with and without a bias.
+enum Scores : int { kPlain = 0, kBiased = 1, kCapped = 2 };
+
+inline Scores scores_of(const AttnParams& p) { return p.cap > 0.f ? kCapped : (p.slopes != nullptr ? kBiased : kPlain); }
+
+// Capped base-2 scores of N raw ones in place.
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreScale& sc) {
+  float far = 0.f;
+#pragma unroll
+  for (int c = 0; c < N; c += 2) far = fmaxf(far, fmaxf(fabsf(s[c]), fabsf(s[c + 1])));
+  // Scores well below the cap, the common case: four or six FMA-pipe operations, two scores at
+  // a time, in place of two MUFU ones, of which an SM has 16 a clock.
+  if (__all_sync(0xffffffffu, far <= sc.near)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const Pair x(s[c], s[c + 1]), u = mul2(x, x);
+      Pair y = fma2(u, Pair(sc.poly3[2], sc.poly3[2]), Pair(sc.poly3[1], sc.poly3[1]));
+      y = fma2(u, y, Pair(sc.poly3[0], sc.poly3[0]));
+      mul2(x, y).split(s[c], s[c + 1]);
+    }
+  } else if (__all_sync(0xffffffffu, far <= sc.mid)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const Pair x(s[c], s[c + 1]), u = mul2(x, x);
+      Pair y = fma2(u, Pair(sc.poly5[4], sc.poly5[4]), Pair(sc.poly5[3], sc.poly5[3]));
+      y = fma2(u, y, Pair(sc.poly5[2], sc.poly5[2]));
+      y = fma2(u, y, Pair(sc.poly5[1], sc.poly5[1]));
+      y = fma2(u, y, Pair(sc.poly5[0], sc.poly5[0]));
+      mul2(x, y).split(s[c], s[c + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) s[c] = tanh_ex2(s[c] * sc.cap_in) * sc.cap_out;
+  }
+}
+
+// s = s * factor - slope |d0 + c| for N scores whose distances are d0, d0 + 1, ...  `slope`: of the
+// bias times log2 e; `side`: -1 when no distance is positive, 1 when none is negative, 0 when both occur.
+template <int N>
+__device__ __forceinline__ void bias_scores(float (&s)[N], float factor, float slope, float d0, int side) {
+  if (side != 0) {
+    const float t = side < 0 ? slope : -slope, base = t * d0;  // the column is an immediate operand
+#pragma unroll
+    for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, fmaf(t, static_cast<float>(c), base));
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, -slope * fabsf(d0 + c));
+  }
+}
+
+// A score that counts as nothing, finite so that products with its zero weight are zero.
+constexpr float kMasked = -1e15f;
+
+// Clears the rows of an operand tile that `dead` names: sub-tiles of 64 columns and ROWS rows.
+template <int ROWS>
+__device__ __forceinline__ void zero_dead_rows(char* tile, int subtiles, const uint32_t (&dead)[ROWS / 32], int lane) {
+#pragma unroll 1
+  for (int r = 0; r < ROWS; ++r) {
+    if (!((dead[r >> 5] >> (r & 31)) & 1u)) continue;
     for (int i = lane; i < subtiles * 8; i += 32)
-      *reinterpret_cast<uint4*>(tile + (i >> 3) * (kAttnTile * 128) + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(tile + (i >> 3) * (ROWS * 128) + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+// Where 16-byte piece `piece` of row `row` lies in a 64-column tile (128-byte swizzle).
+__device__ __forceinline__ char* swizzled(char* tile, int row, int piece) {
+  return tile + row * 128 + ((piece ^ (row & 7)) << 4);
+}
+
+// 32 fp32 values as four 16-byte pieces of T, from piece `first` on, into a staged row; with
+// LOW also what the rounding took, into the same place of a second tile.
+template <typename T, bool LOW>
+__device__ __forceinline__ void stage_row(char* tile, char* low, int row, int first, const float (&o)[32]) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 8) {
+    uint4 w;
+    uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) wp[k] = pack2<T>(o[e + 2 * k], o[e + 2 * k + 1]);
+    *reinterpret_cast<uint4*>(swizzled(tile, row, first + e / 8)) = w;
+    if (LOW) {
+      const T* hi = reinterpret_cast<const T*>(&w);
+      uint4 v;
+      uint32_t* vp = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        vp[k] = pack2<T>(o[e + 2 * k] - to_f32<T>(hi[2 * k]), o[e + 2 * k + 1] - to_f32<T>(hi[2 * k + 1]));
+      *reinterpret_cast<uint4*>(swizzled(low, row, first + e / 8)) = v;
+    }
   }
 }
 

@@ -36,6 +36,7 @@ constexpr int kHalf = kAttnTile / 2;
 
 struct BwdParams {
   AttnParams a;
+  ScoreScale sc;
   int nq, nk;
   int* status;
 };
@@ -89,32 +90,27 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uin
     mma_ts(d, a + (k / 4) * HALF + (k % 4) * 8, smem_desc(b + k * 2048, kAttnTile * 128, 1024), desc, add || k > 0);
 }
 
-// Writes `cols` fp32 columns of TMEM as T, times f: one row of a [.., D] tensor.
+// COLS fp32 columns of TMEM (from `col` on) as T, times f, into a staged tile of 128 rows.
 template <typename T, int COLS>
-__device__ __forceinline__ void store_tmem_row(uint32_t addr, T* dst, int col0, int d, float f, bool valid, bool some,
-                                               bool ok) {
+__device__ __forceinline__ void stage_tmem_row(uint32_t addr, char* tile, int row, int col, float f, bool some, bool ok) {
 #pragma unroll
-  for (int c = 0; c < COLS / 32; ++c) {
+  for (int c = 0; c < COLS; c += 32) {
     float o[32];
     if (some && ok) {
-      tmem_ld32(addr + c * 32, reinterpret_cast<uint32_t*>(o));
+      tmem_ld32(addr + c, reinterpret_cast<uint32_t*>(o));
       tmem_wait_ld();
     }
-    if (!valid) continue;
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      if (col0 + c * 32 + e >= d) continue;
-      uint4 w;
-      uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float x = !ok ? __int_as_float(0x7fc00000) : (some ? o[e + 2 * k] * f : 0.f);
-        const float y = !ok ? __int_as_float(0x7fc00000) : (some ? o[e + 2 * k + 1] * f : 0.f);
-        wp[k] = pack2<T>(x, y);
-      }
-      *reinterpret_cast<uint4*>(dst + col0 + c * 32 + e) = w;
-    }
+    for (int e = 0; e < 32; ++e) o[e] = !ok ? __int_as_float(0x7fc00000) : (some ? o[e] * f : 0.f);
+    stage_row<T, false>(tile + (col + c) / 64 * (kAttnTile * 128), nullptr, row, (col + c) % 64 / 8, o);
   }
+}
+
+// A staged tile to global memory, once all compute threads have written their part.
+template <int D>
+__device__ __forceinline__ void store_tile(const CUtensorMap* m, const char* tile, int row, int h, int b) {
+  for (int c = 0; c < D / 64; ++c) tma_store_4d(m, tile + c * kAttnTile * 128, c * 64, row, h, b);
+  bulk_commit();
 }
 
 // --- row statistics ---------------------------------------------------------------------------------------------
@@ -155,28 +151,11 @@ __global__ void __launch_bounds__(256) stats_kernel(const BwdParams bp) {
 
 // --- dq ---------------------------------------------------------------------------------------------------------
 
-// Base-2 score of a raw one, and the cap's factor on its gradient.
-template <bool GENERAL>
-__device__ __forceinline__ float base2_score(float s, const ScoreScale& sc, bool capped, bool biased, float dist, float* f) {
-  if (!GENERAL) return s * sc.c;
-  float x;
-  if (capped) {
-    const float t = tanh_ex2(s * sc.cap_in);
-    x = t * sc.cap_out;
-    *f = fmaf(-t, t, 1.f);
-  } else {
-    x = s * sc.c;
-    *f = 1.f;
-  }
-  if (biased) x = fmaf(-sc.slope, fabsf(dist), x);
-  return x;
-}
-
-template <typename T, int D, bool GENERAL>
+template <typename T, int D, Scores MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
               const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-              const __grid_constant__ BwdParams bp) {
+              const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ BwdParams bp) {
   using S = Shape<D>;
   constexpr int kColS = 0, kColDP = 128, kColDQ = 256, kColDS = 384;  // dS: 64 columns of its own
   const AttnParams& p = bp.a;
@@ -199,40 +178,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int4 tr = attn_tile_range(p, b, qt);
   const int t0 = tr.x / kAttnTile, n = max(0, (tr.y + kAttnTile - 1) / kAttnTile - t0);
 
+  auto load = [&](int j) {
+    const int st = j % S::kStages;
+    char* dst = skv + st * 2 * S::kTileBytes;
+    mbar_arrive_expect_tx(&bar.full[st], 2 * S::kTileBytes);
+    for (int c = 0; c < D / 64; ++c) {
+      tma_load_4d(dst + c * kAttnTile * 128, &map_k, &bar.full[st], c * 64, (t0 + j) * kAttnTile, kv_head, b);
+      tma_load_4d(dst + S::kTileBytes + c * kAttnTile * 128, &map_v, &bar.full[st], c * 64, (t0 + j) * kAttnTile, kv_head, b);
+    }
+  };
   if (warp == 9) {
     tmem_alloc(&tmem_slot, 512);
-  } else if (threadIdx.x == kCompute) {
-    prefetch_tensor_map(&map_q);
-    prefetch_tensor_map(&map_do);
-    prefetch_tensor_map(&map_k);
-    prefetch_tensor_map(&map_v);
-    raised = 0;
-    init_barriers(bar);
+  } else if (warp == 8) {  // the first copies are under way before the block meets
+    if (elect_one()) {
+      raised = 0;
+      init_barriers(bar);
+      if (n > 0) {
+        mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(sq + c * kAttnTile * 128, &map_q, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
+          tma_load_4d(sdo + c * kAttnTile * 128, &map_do, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
+        }
+        for (int j = 0; j < min(n, S::kStages); ++j) load(j);
+      }
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const Guard guard{&raised, bp.status};
+  bool ok = true;
 
   if (warp == 8) {
     if (n > 0 && elect_one()) {
-      mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_4d(sq + c * kAttnTile * 128, &map_q, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
-        tma_load_4d(sdo + c * kAttnTile * 128, &map_do, &bar.fixed_full, c * 64, qt * kAttnTile, h, b);
-      }
-      int j = 0;
+      int j = min(n, S::kStages);
       for (; j < n; ++j) {
-        const int st = j % S::kStages, ph = (j / S::kStages) & 1;
-        if (!guard.wait(&bar.empty[st], ph ^ 1)) break;
-        char* dst = skv + st * 2 * S::kTileBytes;
-        mbar_arrive_expect_tx(&bar.full[st], 2 * S::kTileBytes);
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(dst + c * kAttnTile * 128, &map_k, &bar.full[st], c * 64, (t0 + j) * kAttnTile, kv_head, b);
-          tma_load_4d(dst + S::kTileBytes + c * kAttnTile * 128, &map_v, &bar.full[st], c * 64, (t0 + j) * kAttnTile,
-                      kv_head, b);
-        }
+        if (!guard.wait(&bar.empty[j % S::kStages], ((j / S::kStages) & 1) ^ 1)) break;
+        load(j);
       }
       if (raised) {  // no copy may be in flight when the block leaves
         Guard::drain(&bar.fixed_full, 0);
@@ -247,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t aq = smem_addr(sq), ado = smem_addr(sdo), akv = smem_addr(skv);
       const uint4* dead = p.plan.kdead != nullptr ? p.plan.kdead + static_cast<int64_t>(b) * bp.nk + t0 : nullptr;
       const bool leader = elect_one();
-      bool ok = guard.wait_warp(&bar.fixed_full, 0);
+      ok = guard.wait_warp(&bar.fixed_full, 0);
       auto stage = [&](int j) { return akv + (j % S::kStages) * 2 * S::kTileBytes; };
       auto arrived = [&](int j) {  // K and V of tile j; padding keys cleared
         ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
@@ -255,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (dead != nullptr) {
           const uint4 w = dead[j];
           if (any_bit(w)) {
-            zero_dead_rows(skv + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), w, lane);
+            zero_dead_rows<kAttnTile>(skv + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), {w.x, w.y, w.z, w.w}, lane);
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -312,38 +296,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool valid = i < p.sq;
     const int2 range = valid ? attn_row_range(p, b, i) : make_int2(0, 0);
     const int pos = i + p.sk - p.sq;
-    const ScoreScale sc = ScoreScale::of(p, h);
+    const float slope = MODE != kPlain && p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
     const float* st = p.stats + ((static_cast<int64_t>(b) * p.hq + h) * bp.nq + qt) * 2 * kAttnTile + r;
     const float nlse = st[0] + prob_shift<T>(), delta = st[kAttnTile];
+    const Pair nlse2(nlse, nlse), delta2(-delta, -delta), c2(bp.sc.c, bp.sc.c);
+    const Pair inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
+    const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
-    bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int key0 = (t0 + j) * kAttnTile + half * kHalf;
       const bool full = tr.z <= key0 && tr.w >= key0 + kHalf;
       if (!(ok = guard.wait_warp(&bar.s_full, j & 1))) break;
       tc_fence_after();
-      float pf[kHalf];  // probability times the cap's factor
+      float pf[kHalf];  // scores, then probability times the cap's factor
       tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
       tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(&bar.s_free);
-      const float d0 = static_cast<float>(key0 - pos);
-#pragma unroll
-      for (int c = 0; c < kHalf; ++c) {
-        float f = 1.f;
-        if (GENERAL) {
-          const float x = base2_score<GENERAL>(pf[c], sc, p.cap > 0.f, p.slopes != nullptr, d0 + c, &f);
-          pf[c] = ex2(x + nlse) * (prob_unshift<T>() * f);
-        } else {
-          pf[c] = ex2(fmaf(pf[c], sc.c, nlse));
-          if (prob_unshift<T>() != 1.f) pf[c] *= prob_unshift<T>();
-        }
-      }
+      if (MODE == kCapped) cap_scores(pf, bp.sc);
       if (!full) {
         const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
 #pragma unroll
-        for (int c = 0; c < kHalf; ++c) pf[c] = from + c < len ? pf[c] : 0.f;
+        for (int c = 0; c < kHalf; ++c) pf[c] = from + c < len ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
+      }
+      const float d0 = static_cast<float>(key0 - pos);
+      // The distance's sign is known (masked pairs do not count): the bias joins the log-sum.
+      const bool behind = MODE != kPlain &&
+                          __all_sync(0xffffffffu, key0 + kHalf - 1 <= pos || (p.causal && p.plan.range == nullptr));
+      if (MODE == kPlain || behind || slope == 0.f) {
+        const float base = fmaf(slope, d0, nlse);
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 2) {
+          const Pair x(pf[c], pf[c + 1]);
+          const Pair add = MODE == kPlain ? nlse2 : Pair(fmaf(slope, static_cast<float>(c), base), fmaf(slope, static_cast<float>(c + 1), base));
+          float e0, e1;
+          (MODE == kCapped ? add2(x, add) : fma2(x, c2, add)).split(e0, e1);
+          Pair e(ex2(e0), ex2(e1));
+          if (MODE == kCapped) {  // 1 - tanh^2, from the score without the bias
+            const Pair u = mul2(x, inv2);
+            e = mul2(e, fma2(mul2(u, minus2), u, one2));
+          }
+          if (prob_unshift<T>() != 1.f) e = mul2(e, unshift2);
+          e.split(pf[c], pf[c + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kHalf; ++c) {
+          const float u = pf[c] * bp.sc.cap_inv, f = MODE == kCapped ? fmaf(-u, u, 1.f) : 1.f;
+          const float x = fmaf(pf[c], MODE == kCapped ? 1.f : bp.sc.c, fmaf(-slope, fabsf(d0 + c), nlse));
+          pf[c] = ex2(x) * (f * prob_unshift<T>());
+        }
       }
       if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
       tc_fence_after();
@@ -353,17 +356,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         float dp[32];
         tmem_ld32(lanes + kColDP + half * kHalf + c * 32, reinterpret_cast<uint32_t*>(dp));
         tmem_wait_ld();
-        if (full) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            w[c * 16 + e / 2] = pack2<T>(pf[c * 32 + e] * (dp[e] - delta), pf[c * 32 + e + 1] * (dp[e + 1] - delta));
-        } else {  // a masked pair is zero, whatever its product is
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float x = pf[c * 32 + e], y = pf[c * 32 + e + 1];
-            w[c * 16 + e / 2] = pack2<T>(x == 0.f ? 0.f : x * (dp[e] - delta), y == 0.f ? 0.f : y * (dp[e + 1] - delta));
-          }
+        for (int e = 0; e < 32; e += 2) {
+          float x, y;
+          mul2(Pair(pf[c * 32 + e], pf[c * 32 + e + 1]), add2(Pair(dp[e], dp[e + 1]), delta2)).split(x, y);
+          dp[e] = x;
+          dp[e + 1] = y;
         }
+        if (!full) {  // a masked pair is zero, whatever its product is
+#pragma unroll
+          for (int e = 0; e < 32; ++e) dp[e] = pf[c * 32 + e] == 0.f ? 0.f : dp[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) w[c * 16 + e / 2] = pack2<T>(dp[e], dp[e + 1]);
       }
       if (j > 0) {  // the last dS has been read
         if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
@@ -378,12 +383,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = guard.wait_warp(&bar.second_done, (n - 1) & 1);
       tc_fence_after();
     }
-    T* dst = static_cast<T*>(p.dq.ptr) + b * p.dq.sb + h * p.dq.sh + i * p.dq.ss;
-    store_tmem_row<T, D / 2>(lanes + kColDQ + half * (D / 2), dst, half * (D / 2), p.d, p.scale, valid, n > 0, ok);
+  }
+  __syncthreads();  // all copies and products are over: Q's place takes the result
+  if (warp < 8) {
+    const int half = warp / 4, row = (warp % 4) * 32 + lane;
+    stage_tmem_row<T, D / 2>(tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + kColDQ + half * (D / 2), sq, row,
+                             half * (D / 2), p.scale, n > 0, ok);
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0) {
+    store_tile<D>(&map_dq, sq, qt * kAttnTile, h, b);
+    bulk_wait_read();
+  }
   if (warp == 9) tmem_free(tmem, 512);
 }
 
@@ -417,10 +431,11 @@ struct RowTiles {
   }
 };
 
-template <typename T, int D, bool GENERAL>
+template <typename T, int D, Scores MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+               const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv,
                const __grid_constant__ BwdParams bp) {
   using S = Shape<D>;
   // D = 64 leaves room for P and dS beside S and dP; else each half of the warps writes
@@ -450,20 +465,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 9) {
     tmem_alloc(&tmem_slot, 512);
-  } else if (threadIdx.x == kCompute) {
-    prefetch_tensor_map(&map_q);
-    prefetch_tensor_map(&map_do);
-    prefetch_tensor_map(&map_k);
-    prefetch_tensor_map(&map_v);
-    raised = 0;
-    first_tile = 0x7fffffff;
-    last_tile = -1;
-    init_barriers(bar);
+  } else if (warp == 8) {  // the first copies are under way before the block meets
+    if (elect_one()) {
+      raised = 0;
+      first_tile = 0x7fffffff;
+      last_tile = -1;
+      init_barriers(bar);
+      mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_4d(sk + c * kAttnTile * 128, &map_k, &bar.fixed_full, c * 64, key0, hk, b);
+        tma_load_4d(sv + c * kAttnTile * 128, &map_v, &bar.fixed_full, c * 64, key0, hk, b);
+      }
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  {  // the first and last row tile that see a key of this tile
+  if (p.plan.tile != nullptr) {  // the first and last row tile that see a key of this tile
     int a = 0x7fffffff, z = -1;
     for (int t = threadIdx.x; t < bp.nq; t += kThreads) {
       const int4 r = attn_tile_range(p, b, t);
@@ -478,20 +497,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       atomicMin(&first_tile, a);
       atomicMax(&last_tile, z);
     }
+    __syncthreads();
   }
-  __syncthreads();
   const uint32_t tmem = tmem_slot;
   const Guard guard{&raised, bp.status};
+  bool ok = true;
   RowTiles it{&p, b, key0, first_tile, last_tile, group, 0, 0, false};
+  if (p.plan.tile == nullptr) {
+    it.first = p.causal ? max(0, key0 - (p.sk - p.sq)) / kAttnTile : 0;
+    it.last = bp.nq - 1;
+  }
   const bool some = it.begin();
 
   if (warp == 8) {
     if (some && elect_one()) {
-      mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_4d(sk + c * kAttnTile * 128, &map_k, &bar.fixed_full, c * 64, key0, hk, b);
-        tma_load_4d(sv + c * kAttnTile * 128, &map_v, &bar.fixed_full, c * 64, key0, hk, b);
-      }
       int j = 0;
       bool more = true;
       for (; more; ++j, more = it.next()) {
@@ -510,10 +529,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           bulk_g2s(rd + 1024, p.plan.range + (static_cast<int64_t>(b) * bp.nq + it.t) * kAttnTile, 1024, &bar.full[st]);
       }
       if (raised) {  // no copy may be in flight when the block leaves
-        Guard::drain(&bar.fixed_full, 0);
         for (int i = max(0, j - S::kStages); i < j; ++i) Guard::drain(&bar.full[i % S::kStages], (i / S::kStages) & 1);
       }
     }
+    if (!some || raised) Guard::drain(&bar.fixed_full, 0);
     __syncwarp();
   } else if (warp == 9) {
     if (some) {
@@ -521,14 +540,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kRows = mma_desc<T>(128, D, false, true);
       const uint32_t ak = smem_addr(sk), av = smem_addr(sv), aqd = smem_addr(sqd);
       const bool leader = elect_one();
-      bool ok = guard.wait_warp(&bar.fixed_full, 0);
+      ok = guard.wait_warp(&bar.fixed_full, 0);
       auto stage = [&](int j) { return aqd + (j % S::kStages) * 2 * S::kTileBytes; };
       auto arrived = [&](int j) {  // Q and dO of step j; rows without keys cleared
         ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
         if (!ok || it.full) return;
         const uint4 w = attn_tile_qdead(p, b, it.t);
         if (any_bit(w)) {
-          zero_dead_rows(sqd + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), w, lane);
+          zero_dead_rows<kAttnTile>(sqd + (j % S::kStages) * 2 * S::kTileBytes, 2 * (D / 64), {w.x, w.y, w.z, w.w}, lane);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -611,8 +630,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int r = (warp % 4) * 32 + lane, half = warp / 4;
     const int key = key0 + r;
+    const Pair c2(bp.sc.c, bp.sc.c), inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
+    const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
-    bool ok = true, more = some;
+    bool more = some;
     int j = 0;
     for (; more; ++j) {
       const int st = j % S::kStages;
@@ -620,48 +641,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int2* range = reinterpret_cast<const int2*>(rows + st * S::kRowBytes + 1024) + half * kHalf;
       const int row0 = it.t * kAttnTile + half * kHalf;
       const bool full = it.full;
-      const ScoreScale sc = ScoreScale::of(p, hk * group + it.g);
+      const float slope = MODE != kPlain && p.slopes != nullptr ? p.slopes[hk * group + it.g] * kLog2e : 0.f;
       more = it.next();
       if (!(ok = guard.wait_warp(&bar.full[st], (j / S::kStages) & 1) && guard.wait_warp(&bar.s_full, j & 1))) break;
       tc_fence_after();
-      float pf[kHalf];  // probability times the cap's factor
+      float pf[kHalf];  // scores, then probability times the cap's factor
       tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
       tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
       tmem_wait_ld();
-      uint32_t w[32];
-      const float d0 = static_cast<float>(row0 + p.sk - p.sq - key);
-      unsigned seen[2] = {0xffffffffu, 0xffffffffu};  // which of the 64 rows see this key
-      if (!full && (p.causal || p.plan.range != nullptr)) {
-        seen[0] = seen[1] = 0u;
+      if (MODE == kCapped) cap_scores(pf, bp.sc);
+      const int first_pos = row0 + p.sk - p.sq;
+      if (!full) {
         if (p.plan.range != nullptr) {
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) {
-            const int2 v = range[c];
-            if (key >= v.x && key < v.y) seen[c / 32] |= 1u << (c % 32);
+          for (int c = 0; c < kHalf; c += 2) {
+            const int4 v = *reinterpret_cast<const int4*>(range + c);
+            pf[c] = key >= v.x && key < v.y ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
+            pf[c + 1] = key >= v.z && key < v.w ? pf[c + 1] : (MODE == kCapped ? kMasked : -INFINITY);
           }
-        } else {  // causal: rows from key - (Sk - Sq) on
-          const int from = key - (row0 + p.sk - p.sq);
+        } else if (p.causal) {  // rows from position `key` on
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c)
-            if (c >= from) seen[c / 32] |= 1u << (c % 32);
+          for (int c = 0; c < kHalf; ++c) pf[c] = c >= key - first_pos ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
         }
       }
+      uint32_t w[32];
+      // Distances are row - key here.  With a known sign (masked pairs do not count) they go two at a time.
+      const float d0 = static_cast<float>(first_pos - key);
+      const bool ahead = MODE != kPlain &&
+                         __all_sync(0xffffffffu, first_pos >= key || (p.causal && p.plan.range == nullptr));
+      const float base = prob_shift<T>() - slope * d0;
+      const Pair shift2(prob_shift<T>(), prob_shift<T>());
 #pragma unroll
       for (int c = 0; c < kHalf; c += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(stats + c);
-        const float nlse[4] = {nl.x, nl.y, nl.z, nl.w};
-        float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float f = 1.f;
-          float x = base2_score<GENERAL>(pf[c + e], sc, p.cap > 0.f, p.slopes != nullptr, d0 + (c + e), &f);
-          x = GENERAL ? x + (nlse[e] + prob_shift<T>()) : fmaf(pf[c + e], sc.c, nlse[e] + prob_shift<T>());
-          pr[e] = ex2(x);
-          if (!full) pr[e] = (seen[c / 32] >> ((c + e) % 32)) & 1u ? pr[e] : 0.f;
-          pf[c + e] = GENERAL || prob_unshift<T>() != 1.f ? pr[e] * (prob_unshift<T>() * f) : pr[e];
+        for (int e = 0; e < 4; e += 2) {
+          const Pair x(pf[c + e], pf[c + e + 1]);
+          Pair add = e == 0 ? Pair(nl.x, nl.y) : Pair(nl.z, nl.w);
+          if (MODE != kPlain) {
+            if (ahead)
+              add = add2(add, Pair(fmaf(-slope, static_cast<float>(c + e), base), fmaf(-slope, static_cast<float>(c + e + 1), base)));
+            else
+              add = add2(add, Pair(fmaf(-slope, fabsf(d0 + (c + e)), prob_shift<T>()),
+                                   fmaf(-slope, fabsf(d0 + (c + e + 1)), prob_shift<T>())));
+          } else if (prob_shift<T>() != 0.f) {
+            add = add2(add, shift2);
+          }
+          float p0, p1;
+          (MODE == kCapped ? add2(x, add) : fma2(x, c2, add)).split(p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          w[(c + e) / 2] = pack2<T>(p0, p1);
+          Pair f(p0, p1);
+          if (MODE == kCapped) {  // 1 - tanh^2, from the score without the bias
+            const Pair u = mul2(x, inv2);
+            f = mul2(f, fma2(mul2(u, minus2), u, one2));
+          }
+          if (prob_unshift<T>() != 1.f) f = mul2(f, unshift2);
+          f.split(pf[c + e], pf[c + e + 1]);
         }
-        w[c / 2] = pack2<T>(pr[0], pr[1]);
-        w[c / 2 + 1] = pack2<T>(pr[2], pr[3]);
       }
       if (kOwn && j > 0) {  // the last P has been read
         if (!(ok = guard.wait_warp(&bar.first_done, (j - 1) & 1))) break;
@@ -681,15 +719,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 dl = *reinterpret_cast<const float4*>(stats + kAttnTile + c * 32 + e);
-          float ds[4] = {dp[e] - dl.x, dp[e + 1] - dl.y, dp[e + 2] - dl.z, dp[e + 3] - dl.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float x = pf[c * 32 + e + k];
-            ds[k] = !full && x == 0.f ? 0.f : x * ds[k];  // a masked pair is zero, whatever its product is
-          }
-          w[c * 16 + e / 2] = pack2<T>(ds[0], ds[1]);
-          w[c * 16 + e / 2 + 1] = pack2<T>(ds[2], ds[3]);
+          mul2(Pair(pf[c * 32 + e], pf[c * 32 + e + 1]), fma2(Pair(dl.x, dl.y), minus2, Pair(dp[e], dp[e + 1]))).split(dp[e], dp[e + 1]);
+          mul2(Pair(pf[c * 32 + e + 2], pf[c * 32 + e + 3]), fma2(Pair(dl.z, dl.w), minus2, Pair(dp[e + 2], dp[e + 3])))
+              .split(dp[e + 2], dp[e + 3]);
         }
+        if (!full) {  // a masked pair is zero, whatever its product is
+#pragma unroll
+          for (int e = 0; e < 32; ++e) dp[e] = pf[c * 32 + e] == 0.f ? 0.f : dp[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) w[c * 16 + e / 2] = pack2<T>(dp[e], dp[e + 1]);
       }
       if (kOwn && j > 0) {  // the last dS has been read
         if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
@@ -704,43 +743,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = guard.wait_warp(&bar.second_done, (j - 1) & 1);
       tc_fence_after();
     }
-    const bool valid = key < p.sk;
-    const int col = half * (D / 2);
-    T* dv = static_cast<T*>(p.dv.ptr) + b * p.dv.sb + hk * p.dv.sh + key * p.dv.ss;
-    T* dk = static_cast<T*>(p.dk.ptr) + b * p.dk.sb + hk * p.dk.sh + key * p.dk.ss;
-    store_tmem_row<T, D / 2>(lanes + kColDV + col, dv, col, p.d, prob_unshift<T>(), valid, some, ok);
-    store_tmem_row<T, D / 2>(lanes + kColDK + col, dk, col, p.d, p.scale, valid, some, ok);
+  }
+  __syncthreads();  // all copies and products are over: the places of K and V take their gradients
+  if (warp < 8) {
+    const int col = warp / 4 * (D / 2), row = (warp % 4) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
+    stage_tmem_row<T, D / 2>(lanes + kColDV + col, sv, row, col, prob_unshift<T>(), some, ok);
+    stage_tmem_row<T, D / 2>(lanes + kColDK + col, sk, row, col, p.scale, some, ok);
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0) {
+    store_tile<D>(&map_dv, sv, key0, hk, b);
+    store_tile<D>(&map_dk, sk, key0, hk, b);
+    bulk_wait_read();
+  }
   if (warp == 9) tmem_free(tmem, 512);
 }
 
-template <typename T, int D, bool GENERAL>
+template <typename T, int D, Scores MODE>
 cudaError_t run(const BwdParams& bp, cudaStream_t s) {
   const AttnParams& p = bp.a;
-  CUtensorMap q, g, k, v;
+  CUtensorMap q, g, k, v, dq, dk, dv;
   if (!attn_map(&q, p.q, p, p.hq, p.sq, kAttnTile, 1) || !attn_map(&g, p.dout, p, p.hq, p.sq, kAttnTile, 1) ||
-      !attn_map(&k, p.k, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, kAttnTile, 1))
+      !attn_map(&k, p.k, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&dq, p.dq, p, p.hq, p.sq, kAttnTile, 1) ||
+      !attn_map(&dk, p.dk, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&dv, p.dv, p, p.hk, p.sk, kAttnTile, 1))
     return cudaErrorInvalidValue;
   constexpr int kLanes = D / 8, kRowsPerBlock = 256 / kLanes;
   const int64_t rows = static_cast<int64_t>(bp.nq) * kAttnTile * p.b * p.hq;
   stats_kernel<T, kLanes><<<static_cast<unsigned>((rows + kRowsPerBlock - 1) / kRowsPerBlock), 256, 0, s>>>(bp);
-  cudaError_t e = cudaFuncSetAttribute(dq_kernel<T, D, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(dq_kernel<T, D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(dkv_kernel<T, D, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  e = cudaFuncSetAttribute(dkv_kernel<T, D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
-  dq_kernel<T, D, GENERAL>
-      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nq) * p.b * p.hq), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, bp);
-  dkv_kernel<T, D, GENERAL>
-      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nk) * p.b * p.hk), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, bp);
+  dq_kernel<T, D, MODE>
+      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nq) * p.b * p.hq), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, dq, bp);
+  dkv_kernel<T, D, MODE>
+      <<<static_cast<unsigned>(static_cast<int64_t>(bp.nk) * p.b * p.hk), kThreads, Shape<D>::kSmem, s>>>(q, g, k, v, dk, dv, bp);
   return cudaGetLastError();
 }
 
 template <typename T, int D>
 cudaError_t by_scores(const BwdParams& bp, cudaStream_t s) {
-  return bp.a.cap > 0.f || bp.a.slopes != nullptr ? run<T, D, true>(bp, s) : run<T, D, false>(bp, s);
+  switch (scores_of(bp.a)) {
+    case kPlain: return run<T, D, kPlain>(bp, s);
+    case kBiased: return run<T, D, kBiased>(bp, s);
+    case kCapped: return run<T, D, kCapped>(bp, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -748,7 +800,7 @@ cudaError_t by_scores(const BwdParams& bp, cudaStream_t s) {
 namespace launch {
 
 cudaError_t attention_tc_backward(const AttnParams& p, cudaStream_t s) {
-  BwdParams bp{p, (p.sq + kAttnTile - 1) / kAttnTile, (p.sk + kAttnTile - 1) / kAttnTile, attn_status_ptr()};
+  BwdParams bp{p, ScoreScale::of(p), (p.sq + kAttnTile - 1) / kAttnTile, (p.sk + kAttnTile - 1) / kAttnTile, attn_status_ptr()};
   if (p.dt == kBF16) return p.d <= 64 ? by_scores<__nv_bfloat16, 64>(bp, s) : by_scores<__nv_bfloat16, 128>(bp, s);
   return p.d <= 64 ? by_scores<__half, 64>(bp, s) : by_scores<__half, 128>(bp, s);
 }

@@ -1,21 +1,20 @@
 // Masked attention forward on the 5th-generation tensor cores.
 //
 // One CTA holds a tile of 128 rows of queries and walks over its visible keys,
-// 128 at a time: S = Q K^T into TMEM, softmax with the running maximum and sum in
-// registers (one thread a row), P as 16-bit values back into TMEM, O += P V with
-// P as the TMEM operand.  S, P and O never leave the SM.
+// KEYS at a time: S = Q K^T into TMEM, softmax with the running maximum and sum in
+// registers, P as 16-bit values back into TMEM over the scores they came from, O += P V
+// with P as the TMEM operand.  S, P and O never leave the SM.
 //
-//   warps 0-3  softmax: row r of the tile is thread r
-//   warp 4     copies: Q once, then K and V tiles through tensor maps
-//   warp 5     issues the MMAs (and clears padding rows of a tile)
+//   softmax warps   a thread takes 64 scores of a row: one warpgroup for 64 keys, two for 128
+//   last warp       copies through tensor maps and MMAs (and clears padding rows of a tile)
 //
 // What bounds it: a score costs one exponential, 16 a clock and SM, and 4 D
 // operations, 8192 a clock and SM, so up to D = 128 the exponentials are the
-// floor (D = 64: twice the MMA time).  Two CTAs share an SM (256 TMEM columns,
-// at most 97 KB each), so one's softmax runs beside the other's MMAs, copies,
-// start and end; registers are moved from the copy warps to the softmax warps so
-// that a row's 128 scores stay in registers between the maximum and the
-// exponentials.
+// floor (D = 64: twice the MMA time).  A warp's way through a tile (wait, TMEM load,
+// maximum, exponentials, TMEM store, wait for the product) is mostly latency, so what
+// counts is how many warps an SM has under way: 16, as four CTAs of 128 TMEM columns for
+// D = 64 and two CTAs of 256 columns for D = 128.  With 8 warps an SM (128 scores a
+// thread) the exponential pipe was busy 54 % of the time.
 //
 // The running maximum is only followed when it grows by more than 4 (a factor of
 // 16 in P), so most tiles do not touch O; the sum uses the same reference, so the
@@ -39,48 +38,56 @@ namespace {
 
 __device__ int attn_status = 0;
 
-constexpr int kThreads = 256;
 constexpr float kFollow = 4.f;
+constexpr int kCols = 64;  // scores of a row that a thread takes
 
-// Q, then KS tiles of K and VS of V.
 template <int D>
 struct Shape {
-  static constexpr int kTileBytes = kAttnTile * D * 2;
-  static constexpr int kStages = D == 64 ? 2 : 1;
-  static constexpr int kSmem = kTileBytes * (1 + 2 * kStages) + 1024;
-  static constexpr bool kOwnP = D == 64;  // P has columns of its own, else it takes S's
-  static constexpr int kColP = kOwnP ? 128 : 0;
-  static constexpr int kColO = D == 64 ? 192 : 128;
+  static constexpr int kKeys = 64;
+  static constexpr int kSoftmax = 128;  // threads
+  static constexpr int kThreads = kSoftmax + 64;
+  static constexpr bool kTmemQ = D == 64;  // D = 128 fills TMEM with S and O
+  static constexpr int kColO = 2 * kKeys, kColQ = kColO + D;
+  static constexpr int kTmem = 256;
+  static constexpr int kQBytes = kTmemQ ? 0 : kAttnTile * D * 2;
+  static constexpr int kTileBytes = kKeys * D * 2;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kSmem = kQBytes + 2 * kStages * kTileBytes + 1024;
 };
 
 struct FwdParams {
   AttnParams a;
+  ScoreScale sc;
   int packed;  // query heads of one key head in one tile
   int tiles_q;
   int* status;
 };
 
 struct Barriers {
-  uint64_t q_full, s_full, s_free, p_full, pv_done, drain;
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t q_full, pv_done, o_full, drain;
+  uint64_t s_full[2], p_full[2];  // by tile parity
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
 };
 
-template <typename T, int D, bool GENERAL>
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, int D, Scores MODE>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 2)
     fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams fp) {
+               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+               const __grid_constant__ CUtensorMap map_lo,
+               const __grid_constant__ FwdParams fp) {
   using S = Shape<D>;
+  constexpr int kKeys = S::kKeys, kStages = S::kStages;
   const AttnParams& p = fp.a;
   extern __shared__ char smem_raw[];
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int raised;
-  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  char* sq = base;
-  char* sk = base + S::kTileBytes;
-  char* sv = sk + S::kStages * S::kTileBytes;
+  char* sq = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* sk = sq + S::kQBytes;
+  char* sv = sk + kStages * S::kTileBytes;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  constexpr int kCopier = S::kSoftmax / 32, kIssuer = kCopier + 1;
   // Tiles with the most keys first: the last rows of a causal mask.
   const int group = p.hq / p.hk;
   const int heads = fp.packed ? p.hk : p.hq;
@@ -91,40 +98,77 @@ __global__ void __launch_bounds__(kThreads, 2)
   id /= heads;
   const int b = id % p.b;
   const int qt = fp.tiles_q - 1 - id / p.b;
-  const int kv_head = fp.packed ? h : h / group;
 
   const int4 tr = [&] {
     if (fp.packed && p.plan.tile == nullptr)  // all rows of the row tile at once
-      return p.causal ? make_int4(0, max(0, p.sk), 0, max(0, p.sk - p.sq + 1)) : make_int4(0, p.sk, 0, p.sk);
+      return p.causal ? make_int4(0, p.sk, 0, max(0, p.sk - p.sq + 1)) : make_int4(0, p.sk, 0, p.sk);
     return attn_tile_range(p, b, qt);
   }();
-  int t0 = tr.x / kAttnTile, t1 = (tr.y + kAttnTile - 1) / kAttnTile;
+  int key_lo = tr.x, key_hi = tr.y;
   if (p.splits > 1) {
-    t0 = max(t0, split * p.split_tiles);
-    t1 = min(t1, (split + 1) * p.split_tiles);
+    key_lo = max(key_lo, split * p.split_tiles * kAttnTile);
+    key_hi = min(key_hi, (split + 1) * p.split_tiles * kAttnTile);
   }
-  const int n = max(0, t1 - t0);
+  const int t0 = key_lo / kKeys;
+  const int n = max(0, (key_hi + kKeys - 1) / kKeys - t0);
+  const int kv_head = fp.packed ? h : h / group;
+  auto load_k = [&](int j) {
+    const int st = j % kStages;
+    mbar_arrive_expect_tx(&bar.k_full[st], S::kTileBytes);
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(sk + st * S::kTileBytes + c * kKeys * 128, &map_k, &bar.k_full[st], c * 64, (t0 + j) * kKeys, kv_head, b);
+  };
+  auto load_v = [&](int j) {
+    const int st = j % kStages;
+    mbar_arrive_expect_tx(&bar.v_full[st], S::kTileBytes);
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(sv + st * S::kTileBytes + c * kKeys * 128, &map_v, &bar.v_full[st], c * 64, (t0 + j) * kKeys, kv_head, b);
+  };
 
-  if (warp == 5) {
-    tmem_alloc(&tmem_slot, 256);
-  } else if (threadIdx.x == 128) {
-    prefetch_tensor_map(&map_q);
-    prefetch_tensor_map(&map_k);
-    prefetch_tensor_map(&map_v);
-    raised = 0;
-    mbar_init(&bar.q_full, 1);
-    mbar_init(&bar.s_full, 1);
-    mbar_init(&bar.s_free, 128);
-    mbar_init(&bar.p_full, 128);
-    mbar_init(&bar.pv_done, 1);
-    mbar_init(&bar.drain, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], 1);
-      mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], 1);
-      mbar_init(&bar.v_empty[i], 1);
+  // Everything that takes long starts before the block meets: TMEM, the first copies, Q.
+  const int r = (warp % 4) * 32 + lane;  // softmax warps: row of the tile
+  const int i = fp.packed ? r % p.sq : qt * kAttnTile + r;
+  const int head = fp.packed ? h * group + r / p.sq : h;
+  const bool valid = fp.packed ? r < group * p.sq : i < p.sq;
+  uint4 q[8];
+  if (warp == kIssuer) {
+    tmem_alloc(&tmem_slot, S::kTmem);
+  } else if (warp == kCopier) {
+    if (elect_one()) {
+      raised = 0;
+      for (int c = 0; c < kStages; ++c) {
+        mbar_init(&bar.k_full[c], 1);
+        mbar_init(&bar.k_empty[c], 1);
+        mbar_init(&bar.v_full[c], 1);
+        mbar_init(&bar.v_empty[c], 1);
+      }
+      mbar_init(&bar.q_full, S::kTmemQ ? S::kSoftmax : 1);
+      mbar_init_fence();
+      if (!S::kTmemQ && n > 0) {
+        mbar_arrive_expect_tx(&bar.q_full, (fp.packed ? group * p.sq : kAttnTile) * D * 2);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(sq + c * kAttnTile * 128, &map_q, &bar.q_full, c * 64, fp.packed ? 0 : qt * kAttnTile,
+                      fp.packed ? h * group : h, b);
+      }
+      for (int j = 0; j < min(n, kStages); ++j) {
+        load_k(j);
+        load_v(j);
+      }
+      mbar_init(&bar.pv_done, 1);
+      mbar_init(&bar.o_full, 1);
+      mbar_init(&bar.drain, 1);
+      for (int c = 0; c < 2; ++c) {
+        mbar_init(&bar.s_full[c], 1);
+        mbar_init(&bar.p_full[c], S::kSoftmax);
+      }
+      mbar_init_fence();
     }
-    mbar_init_fence();
+    __syncwarp();
+  } else if (S::kTmemQ && n > 0) {  // Q is the TMEM operand of S
+    const T* src = static_cast<const T*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + i * p.q.ss;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      q[c] = valid && c * 8 < p.d ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -132,106 +176,96 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = tmem_slot;
   const Guard guard{&raised, fp.status};
 
-  if (warp >= 4) {
-    regs_down<56>();
-    if (warp == 4 && n > 0) {
-      if (elect_one()) {
-        const int rows_q = fp.packed ? group * p.sq : kAttnTile;  // rows of the tensor map's box
-        mbar_arrive_expect_tx(&bar.q_full, rows_q * D * 2);
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sq + c * kAttnTile * 128, &map_q, &bar.q_full, c * 64, fp.packed ? 0 : qt * kAttnTile,
-                      fp.packed ? h * group : h, b);
-        int j = 0;
-        for (; j < n; ++j) {
-          const int st = j % S::kStages, ph = (j / S::kStages) & 1;
-          if (!guard.wait(&bar.k_empty[st], ph ^ 1)) break;
-          mbar_arrive_expect_tx(&bar.k_full[st], S::kTileBytes);
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sk + st * S::kTileBytes + c * kAttnTile * 128, &map_k, &bar.k_full[st], c * 64,
-                        (t0 + j) * kAttnTile, kv_head, b);
-          if (!guard.wait(&bar.v_empty[st], ph ^ 1)) {  // K of this tile is on its way, V is not
-            Guard::drain(&bar.k_full[st], ph);
-            break;
-          }
-          mbar_arrive_expect_tx(&bar.v_full[st], S::kTileBytes);
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sv + st * S::kTileBytes + c * kAttnTile * 128, &map_v, &bar.v_full[st], c * 64,
-                        (t0 + j) * kAttnTile, kv_head, b);
-        }
-        // No copy may be in flight when the block leaves: the last ones of each stage.
-        if (raised) {
-          Guard::drain(&bar.q_full, 0);
-          for (int i = max(0, j - S::kStages); i < j; ++i) {
-            Guard::drain(&bar.k_full[i % S::kStages], (i / S::kStages) & 1);
-            Guard::drain(&bar.v_full[i % S::kStages], (i / S::kStages) & 1);
-          }
-        }
+  if (warp == kCopier) {
+    if (n > 0 && elect_one()) {
+      int k_loads = min(n, kStages), v_loads = k_loads;
+      for (int j = kStages; j < n; ++j) {
+        const int st = j % kStages, ph = (j / kStages) & 1;
+        if (!guard.wait(&bar.k_empty[st], ph ^ 1)) break;
+        load_k(j);
+        ++k_loads;
+        if (!guard.wait(&bar.v_empty[st], ph ^ 1)) break;
+        load_v(j);
+        ++v_loads;
       }
-      __syncwarp();
-    } else if (warp == 5 && n > 0) {
-      constexpr uint32_t kQK = mma_desc<T>(128, 128, false, false);
+      if (raised) {  // no copy may be in flight when the block leaves
+        if (!S::kTmemQ) Guard::drain(&bar.q_full, 0);
+        for (int i = max(0, k_loads - kStages); i < k_loads; ++i) Guard::drain(&bar.k_full[i % kStages], (i / kStages) & 1);
+        for (int i = max(0, v_loads - kStages); i < v_loads; ++i) Guard::drain(&bar.v_full[i % kStages], (i / kStages) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kIssuer) {
+    if (n > 0) {
+      constexpr uint32_t kQK = mma_desc<T>(128, kKeys, false, false);
       constexpr uint32_t kPV = mma_desc<T>(128, D, false, true);
-      const uint32_t aq = smem_addr(sq), ak = smem_addr(sk), av = smem_addr(sv);
-      const int nk = (p.sk + kAttnTile - 1) / kAttnTile;
-      const uint4* dead = p.plan.kdead != nullptr ? p.plan.kdead + static_cast<int64_t>(b) * nk + t0 : nullptr;
-      const bool leader = elect_one();
-      bool ok = guard.wait_warp(&bar.q_full, 0);
-      // S of tile j; padding keys are cleared first, whatever they hold.
-      auto scores = [&](int j) {
-        const int st = j % S::kStages;
-        if (!(ok = ok && guard.wait_warp(&bar.k_full[st], (j / S::kStages) & 1))) return;
-        if (dead != nullptr) {
-          const uint4 w = dead[j];
-          if (any_bit(w)) {
-            zero_dead_rows(sk + st * S::kTileBytes, D / 64, w, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
+      const uint64_t dq = smem_desc(smem_addr(sq), 16, 1024), dk = smem_desc(smem_addr(sk), 16, 1024),
+                     dv = smem_desc(smem_addr(sv), kKeys * 128, 1024);
+      // Padding keys are cleared, whatever they hold.
+      auto clear_dead = [&](char* tile, int j) {
+        const int first = (t0 + j) * kKeys;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(
+                                  &p.plan.kdead[static_cast<int64_t>(b) * ((p.sk + kAttnTile - 1) / kAttnTile) + first / kAttnTile]) +
+                              first % kAttnTile / 32;
+        uint32_t w[kKeys / 32], any = 0;
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) any |= w[i] = src[i];
+        if (any != 0u) {
+          zero_dead_rows<kKeys>(tile, D / 64, w, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
         }
-        tc_fence_after();
-        if (leader) {
+      };
+      bool ok = guard.wait_warp(&bar.q_full, 0);
+      auto k_ready = [&](int j) {
+        const int st = j % kStages;
+        ok = ok && guard.wait_warp(&bar.k_full[st], (j / kStages) & 1);
+        if (ok && p.plan.kdead != nullptr) clear_dead(sk + st * S::kTileBytes, j);
+      };
+      auto scores = [&](int j) {
+        if (elect_one()) {
+          const uint64_t d = dk + (j % kStages) * (S::kTileBytes / 16);
+#pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * kAttnTile * 128 + (k % 4) * 32;
-            mma_ss(tmem, smem_desc(aq + off, 16, 1024), smem_desc(ak + st * S::kTileBytes + off, 16, 1024), kQK, k > 0);
+            const uint64_t dkk = d + ((k / 4) * kKeys * 128 + (k % 4) * 32) / 16;
+            if (S::kTmemQ)
+              mma_ts(tmem + (j & 1) * kKeys, tmem + S::kColQ + k * 8, dkk, kQK, k > 0);
+            else
+              mma_ss(tmem + (j & 1) * kKeys, dq + ((k / 4) * kAttnTile * 128 + (k % 4) * 32) / 16, dkk, kQK, k > 0);
           }
-          mma_commit(&bar.k_empty[st]);
-          mma_commit(&bar.s_full);
+          mma_commit(&bar.k_empty[j % kStages]);
+          mma_commit(&bar.s_full[j & 1]);
         }
         __syncwarp();
       };
-      scores(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (S::kOwnP && j + 1 < n) {
-          if (!(ok = guard.wait_warp(&bar.s_free, j & 1))) break;
-          scores(j + 1);
-        }
-        const int st = j % S::kStages;
-        if (!(ok = ok && guard.wait_warp(&bar.v_full[st], (j / S::kStages) & 1))) break;
-        if (dead != nullptr) {
-          const uint4 w = dead[j];
-          if (any_bit(w)) {
-            zero_dead_rows(sv + st * S::kTileBytes, D / 64, w, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-        }
-        if (!(ok = guard.wait_warp(&bar.p_full, j & 1))) break;
+      for (int j = 0; j < 2 && j < n; ++j) {
+        k_ready(j);
         tc_fence_after();
-        if (leader) {
-          for (int k = 0; k < kAttnTile / 16; ++k)
-            mma_ts(tmem + S::kColO, tmem + S::kColP + k * 8,
-                   smem_desc(av + st * S::kTileBytes + k * 2048, kAttnTile * 128, 1024), kPV, j > 0 || k > 0);
+        if (ok) scores(j);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int st = j % kStages;
+        if (!(ok = guard.wait_warp(&bar.v_full[st], (j / kStages) & 1))) break;
+        if (p.plan.kdead != nullptr) clear_dead(sv + st * S::kTileBytes, j);
+        if (!(ok = guard.wait_warp(&bar.p_full[j & 1], (j / 2) & 1))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t d = dv + st * (S::kTileBytes / 16);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            mma_ts(tmem + S::kColO, tmem + (j & 1) * kKeys + k * 8, d + k * 128, kPV, j > 0 || k > 0);
           mma_commit(&bar.v_empty[st]);
-          mma_commit(&bar.pv_done);
+          mma_commit(j + 1 < n ? &bar.pv_done : &bar.o_full);
         }
         __syncwarp();
-        if (!S::kOwnP && j + 1 < n) {  // the next S overwrites this P
-          if (!(ok = guard.wait_warp(&bar.pv_done, j & 1))) break;
-          scores(j + 1);
+        if (j + 2 < n) {  // its S takes the place of this P
+          k_ready(j + 2);
+          if (!(ok = ok && guard.wait_warp(&bar.pv_done, j & 1))) break;
+          scores(j + 2);
         }
       }
       if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (leader) {
+        if (elect_one()) {
           mma_commit(&bar.drain);
           Guard::drain(&bar.drain, 0);
         }
@@ -239,113 +273,109 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   } else {
-    regs_up<200>();
-    const int r = threadIdx.x;
-    const int i = fp.packed ? r % p.sq : qt * kAttnTile + r;
-    const int head = fp.packed ? h * group + r / p.sq : h;
-    const bool valid = fp.packed ? r < group * p.sq : i < p.sq;
     const int2 range = valid ? attn_row_range(p, b, i) : make_int2(0, 0);
     const bool warp_works = __any_sync(0xffffffffu, range.y > range.x);
     const int pos = i + p.sk - p.sq;
-    const ScoreScale sc = ScoreScale::of(p, valid ? head : 0);
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const float slope = MODE != kPlain && p.slopes != nullptr ? p.slopes[valid ? head : 0] * kLog2e : 0.f;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    if (S::kTmemQ && n > 0) {
+      tmem_st32(lanes + S::kColQ, reinterpret_cast<const uint32_t*>(q));
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.q_full);
+    }
     for (int j = 0; j < n; ++j) {
-      if (!(ok = guard.wait_warp(&bar.s_full, j & 1))) break;
+      const uint32_t col_s = lanes + (j & 1) * kKeys;
+      if (!(ok = guard.wait_warp(&bar.s_full[j & 1], (j / 2) & 1))) break;
       tc_fence_after();
       if (!warp_works) {  // rows of no use: their P is never looked at
-        if (S::kOwnP) mbar_arrive(&bar.s_free);
-        if (j > 0 && !(ok = guard.wait_warp(&bar.pv_done, (j - 1) & 1))) break;
-        mbar_arrive(&bar.p_full);
+        mbar_arrive(&bar.p_full[j & 1]);
         continue;
       }
-      const int key0 = (t0 + j) * kAttnTile;
-      float s[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(lanes + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+      const int key0 = (t0 + j) * kKeys;
+      float s[kCols];
+      tmem_ld32(col_s, reinterpret_cast<uint32_t*>(s));
+      tmem_ld32(col_s + 32, reinterpret_cast<uint32_t*>(s) + 32);
       tmem_wait_ld();
-      if (S::kOwnP) {
-        tc_fence_before();
-        mbar_arrive(&bar.s_free);
+      if (MODE == kCapped) cap_scores(s, fp.sc);
+      if (MODE == kBiased || (MODE == kCapped && slope != 0.f)) {
+        const bool behind = __all_sync(0xffffffffu, key0 + kCols - 1 <= pos);
+        bias_scores(s, MODE == kBiased ? fp.sc.c : 1.f, slope, static_cast<float>(key0 - pos), behind ? -1 : 0);
       }
-      if (GENERAL) {  // base-2 scores in place
-        if (p.cap > 0.f) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = tanh_ex2(s[c] * sc.cap_in) * sc.cap_out;
-        } else {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] *= sc.c;
-        }
-        if (p.slopes != nullptr) {
-          const float d0 = static_cast<float>(key0 - pos);
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = fmaf(-sc.slope, fabsf(d0 + c), s[c]);
-        }
-      }
-      if (!(tr.z <= key0 && tr.w >= key0 + kAttnTile)) {
+      if (!(tr.z <= key0 && tr.w >= key0 + kCols)) {
         const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = from + c < len ? s[c] : -INFINITY;
+        for (int c = 0; c < kCols; ++c) s[c] = from + c < len ? s[c] : -INFINITY;
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < 128; c += 4)
+      for (int c = 4; c < kCols - 4; c += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[c + e]);
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[c + e]), s[c + 4 + e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[kCols - 4 + e]);
       float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (!GENERAL) best *= sc.c;  // the factor is positive
-      // P of the last tile has to be read, and O to be whole, before either is written.
-      if (j > 0) {
-        if (!(ok = guard.wait_warp(&bar.pv_done, (j - 1) & 1))) break;
-        tc_fence_after();
-      }
+      if (MODE == kPlain) best *= fp.sc.c;  // the factor is positive
       if (__any_sync(0xffffffffu, best > m + kFollow)) {
         const float mn = fmaxf(m, best);
         const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
         m = mn;
         l *= f;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(lanes + S::kColO + c * 32, o);
+        if (j > 0) {  // S(j) came after the product j - 2: j - 1 is the one to wait for
+          if (!(ok = guard.wait_warp(&bar.pv_done, (j - 1) & 1))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t at = lanes + S::kColO + c * 8;
+            uint32_t o[8];
+            tmem_ld8(at, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(lanes + S::kColO + c * 32, o);
+            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st8(at, o);
           }
         }
       }
-      const float ref = (m == -INFINITY ? 0.f : m) - prob_shift<T>();
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float ref = prob_shift<T>() - (m == -INFINITY ? 0.f : m);
+      const Pair ref2(ref, ref), c2(fp.sc.c, fp.sc.c);
+      Pair sum[2] = {Pair(0.f, 0.f), Pair(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int at = c * 32 + e * 2;
-          const float x = ex2(GENERAL ? s[at] - ref : fmaf(s[at], sc.c, -ref));
-          const float y = ex2(GENERAL ? s[at + 1] - ref : fmaf(s[at + 1], sc.c, -ref));
-          sum[e & 3] += x + y;
+          const Pair v(s[c * 32 + e * 2], s[c * 32 + e * 2 + 1]);
+          float x, y;
+          (MODE != kPlain ? add2(v, ref2) : fma2(v, c2, ref2)).split(x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[e & 1] = add2(sum[e & 1], Pair(x, y));
           w[e] = pack2<T>(x, y);
         }
-        tmem_st16(lanes + S::kColP + c * 16, w);
+        tmem_st16(col_s + c * 16, w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float even, odd;
+      add2(sum[0], sum[1]).split(even, odd);
+      l += even + odd;
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&bar.p_full);
+      mbar_arrive(&bar.p_full[j & 1]);
     }
     if (ok && n > 0) {
-      ok = guard.wait_warp(&bar.pv_done, (n - 1) & 1);
+      ok = guard.wait_warp(&bar.o_full, 0);
       tc_fence_after();
     }
     // A row that sees nothing is zero; after a wait that ran out, rows are NaN.
     const bool none = l == 0.f && m == -INFINITY;
     const float f = !ok ? __int_as_float(0x7fc00000) : (none ? 0.f : 1.f / l);
     const int64_t row = (static_cast<int64_t>(b) * p.hq + head) * p.sq + i;
-    if (warp_works || n == 0 || !ok || __any_sync(0xffffffffu, valid)) {
+    const bool staged = ok && !fp.packed && p.splits == 1;
+    // The copies are done and read by now, their place takes the warp's 32 rows, sub-tiles of 64 columns.
+    char* tile = sk + warp * 4096 * (D / 64);
+    char* low = tile + kAttnTile * D * 2;
+    if (__any_sync(0xffffffffu, valid)) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
@@ -355,33 +385,44 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = (n > 0 && !none) || !ok ? (ok ? o[e] : 1.f) * f : 0.f;
-        if (!valid) continue;
-        if (p.splits > 1) {
-          float* dst = p.part_o + (split * (static_cast<int64_t>(p.b) * p.hq * p.sq) + row) * p.d + c * 32;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (c * 32 + e < p.d) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else {
-          const int64_t at = b * p.o.sb + head * p.o.sh + i * p.o.ss + c * 32;
+        if (staged) {
+          if (p.lo.ptr != nullptr)
+            stage_row<T, true>(tile + c / 2 * 4096, low + c / 2 * 4096, lane, c % 2 * 4, o);
+          else
+            stage_row<T, false>(tile + c / 2 * 4096, low + c / 2 * 4096, lane, c % 2 * 4, o);
+        } else if (valid) {  // few rows: straight from the thread
+          const int col = c * 32;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
-            if (c * 32 + e >= p.d) continue;
-            uint4 w;
-            uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+            if (col + e >= p.d) continue;
+            if (p.splits > 1) {
+              float* dst = p.part_o + (split * (static_cast<int64_t>(p.b) * p.hq * p.sq) + row) * p.d + col + e;
+              *reinterpret_cast<float4*>(dst) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              *reinterpret_cast<float4*>(dst + 4) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+            } else {
+              const int64_t at = b * p.o.sb + head * p.o.sh + i * p.o.ss + col + e;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) wp[k] = pack2<T>(o[e + 2 * k], o[e + 2 * k + 1]);
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.o.ptr) + at + e) = w;
-            if (p.lo.ptr != nullptr) {
-              const T* hi = reinterpret_cast<const T*>(&w);
-              uint4 v;
-              uint32_t* vp = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                vp[k] = pack2<T>(o[e + 2 * k] - to_f32<T>(hi[2 * k]), o[e + 2 * k + 1] - to_f32<T>(hi[2 * k + 1]));
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.lo.ptr) + at + e) = v;
+              for (int k = 0; k < 8; ++k) {
+                const T hi = from_f32<T>(o[e + k]);
+                static_cast<T*>(p.o.ptr)[at + k] = hi;
+                if (p.lo.ptr != nullptr) static_cast<T*>(p.lo.ptr)[at + k] = from_f32<T>(o[e + k] - to_f32<T>(hi));
+              }
             }
           }
         }
+      }
+      if (staged) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one()) {
+          for (int c = 0; c < D / 64; ++c) {
+            tma_store_4d(&map_o, tile + c * 4096, c * 64, qt * kAttnTile + warp * 32, head, b);
+            if (p.lo.ptr != nullptr) tma_store_4d(&map_lo, low + c * 4096, c * 64, qt * kAttnTile + warp * 32, head, b);
+          }
+          bulk_commit();
+          bulk_wait_read();
+        }
+        __syncwarp();
       }
     }
     if (valid) {
@@ -395,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_free(tmem, 256);
+  if (warp == kIssuer) tmem_free(tmem, S::kTmem);
 }
 
 // Joins the splits of a row: sum of 2^(lse_s - max) o_s over their sum.  One warp a row.
@@ -435,19 +476,22 @@ __global__ void __launch_bounds__(128) join_kernel(const FwdParams fp) {
   if (lane == 0 && p.lse != nullptr) p.lse[row] = none ? INFINITY : m + log2f(total);
 }
 
-template <typename T, int D, bool GENERAL>
+template <typename T, int D, Scores MODE>
 cudaError_t run(const FwdParams& fp, cudaStream_t s) {
   const AttnParams& p = fp.a;
-  CUtensorMap q, k, v;
-  const int group = p.hq / p.hk;
-  if (!attn_map(&q, p.q, p, p.hq, p.sq, fp.packed ? p.sq : kAttnTile, fp.packed ? group : 1) ||
-      !attn_map(&k, p.k, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, kAttnTile, 1))
+  CUtensorMap q{}, k, v, o{}, lo{};
+  if (!Shape<D>::kTmemQ && !attn_map(&q, p.q, p, p.hq, p.sq, fp.packed ? p.sq : kAttnTile, fp.packed ? p.hq / p.hk : 1))
     return cudaErrorInvalidValue;
-  const auto kernel = fwd_kernel<T, D, GENERAL>;
+  if (!fp.packed && p.splits == 1 &&
+      (!attn_map(&o, p.o, p, p.hq, p.sq, 32, 1) || (p.lo.ptr != nullptr && !attn_map(&lo, p.lo, p, p.hq, p.sq, 32, 1))))
+    return cudaErrorInvalidValue;
+  if (!attn_map(&k, p.k, p, p.hk, p.sk, Shape<D>::kKeys, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, Shape<D>::kKeys, 1))
+    return cudaErrorInvalidValue;
+  const auto kernel = fwd_kernel<T, D, MODE>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t blocks = static_cast<int64_t>(fp.tiles_q) * p.b * (fp.packed ? p.hk : p.hq) * p.splits;
-  kernel<<<static_cast<unsigned>(blocks), kThreads, Shape<D>::kSmem, s>>>(q, k, v, fp);
+  kernel<<<static_cast<unsigned>(blocks), Shape<D>::kThreads, Shape<D>::kSmem, s>>>(q, k, v, o, lo, fp);
   if (p.splits > 1) {
     const int64_t rows = static_cast<int64_t>(p.b) * p.hq * p.sq;
     join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, s>>>(fp);
@@ -457,7 +501,12 @@ cudaError_t run(const FwdParams& fp, cudaStream_t s) {
 
 template <typename T, int D>
 cudaError_t by_scores(const FwdParams& fp, cudaStream_t s) {
-  return fp.a.cap > 0.f || fp.a.slopes != nullptr ? run<T, D, true>(fp, s) : run<T, D, false>(fp, s);
+  switch (scores_of(fp.a)) {
+    case kPlain: return run<T, D, kPlain>(fp, s);
+    case kBiased: return run<T, D, kBiased>(fp, s);
+    case kCapped: return run<T, D, kCapped>(fp, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 bool packs(const AttnParams& p) { return p.hq > p.hk && p.hq / p.hk * p.sq <= kAttnTile; }
@@ -514,6 +563,7 @@ void attention_tc_splits(const AttnParams& p, int sms, int* splits, int* split_t
 cudaError_t attention_tc_forward(const AttnParams& p, cudaStream_t s) {
   FwdParams fp{};
   fp.a = p;
+  fp.sc = ScoreScale::of(p);
   fp.packed = packs(p);
   fp.tiles_q = fp.packed ? 1 : (p.sq + kAttnTile - 1) / kAttnTile;
   fp.status = attn_status_ptr();

@@ -32,27 +32,26 @@ namespace bitscom_b200 {
 // all other waits of the block then return too; the kernel leaves its loops,
 // waits for its own copies, frees its TMEM and returns.
 // ---------------------------------------------------------------------------
-constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr long long kWaitLimitClocks = 8000000000ll;  // about 4 s
 
 struct Guard {
   volatile int* raised;  // shared memory
   int* status;           // global memory
 
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
-    if (mbar_try_wait(bar, parity)) return true;
-    uint64_t start = 0;
-    for (int i = 0;; ++i) {
-      if (mbar_try_wait(bar, parity)) return true;
-      if ((i & 15) == 15) {
-        if (*raised) return false;
-        const uint64_t now = globaltimer_ns();
-        if (start == 0) {
-          start = now;
-        } else if (now - start > kWaitLimitNs) {
-          *raised = 1;
-          atomicExch(status, 1);
-          return false;
-        }
+    return mbar_try_wait(bar, parity) || wait_long(bar, parity);
+  }
+  // The SM's clock, as %globaltimer takes longer to read than most waits last.
+  __device__ __forceinline__ bool wait_long(uint64_t* bar, uint32_t parity) const {
+    const long long start = clock64();
+    for (;;) {
+      for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+      if (*raised) return false;
+      if (clock64() - start > kWaitLimitClocks) {
+        *raised = 1;
+        atomicExch(status, 1);
+        return false;
       }
     }
   }
@@ -62,9 +61,9 @@ struct Guard {
   }
   // After the flag: for copies in flight, whose barriers complete by themselves.
   __device__ __forceinline__ static void drain(uint64_t* bar, uint32_t parity) {
-    const uint64_t start = globaltimer_ns();
+    const long long start = clock64();
     while (!mbar_try_wait(bar, parity))
-      if (globaltimer_ns() - start > kWaitLimitNs) return;
+      if (clock64() - start > kWaitLimitClocks) return;
   }
 };
 
@@ -82,6 +81,17 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uin
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+
+// Shared to global through a tensor map (what lies outside the tensor is not written); to
+// be followed by bulk_commit() and, before the block leaves, bulk_wait_read().
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -124,6 +134,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
@@ -198,6 +218,29 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations an instruction.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void split(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
