@@ -16,8 +16,8 @@
 // and K lie in shared memory once and are read along their columns by the first
 // products and along their rows by the second ones.
 //
-//   warps 0-7  arithmetic: thread = one lane of TMEM, half the 128 columns
-//   warp 8     copies, warp 9 MMAs
+//   warps 0-15 arithmetic: a thread has one lane of TMEM and a quarter of the 128 columns
+//   warp 16    copies, warp 17 MMAs
 //
 // The MMAs of the next tile's S and dP are issued as soon as the arithmetic has read
 // (or, where P and dS share their columns, the second product has read) the present
@@ -30,9 +30,10 @@
 namespace bitscom_b200 {
 namespace {
 
-constexpr int kCompute = 256;
+constexpr int kCompute = 512;
 constexpr int kThreads = kCompute + 64;
-constexpr int kHalf = kAttnTile / 2;
+constexpr int kPart = 32;  // of the 128 columns: a thread's share
+constexpr int kCopier = kCompute / 32, kIssuer = kCopier + 1;
 
 struct BwdParams {
   AttnParams a;
@@ -74,21 +75,31 @@ __device__ __forceinline__ void init_barriers(Barriers& bar) {
   mbar_init_fence();
 }
 
-// One product of a tile along its columns: 128 x 128 scores, contraction over D.
+// The products, from descriptors of whole tiles (an instruction takes 16 values of the
+// contraction; addresses in a descriptor count 16 bytes).  Called by one elected thread of a
+// converged warp with values that are the same for the whole warp: then an
+// instruction issues every 44 (128 x 64, TMEM operand) to 104 clocks (128 x 128, both
+// operands in shared memory), its own time; descriptors built a thread at a time double that.
+//
+// Along the columns of both: 128 x 128, contraction over D.
 template <int D>
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t desc) {
+__device__ __forceinline__ void mma_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t desc) {
+#pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    const uint32_t off = (k / 4) * kAttnTile * 128 + (k % 4) * 32;
-    mma_ss(d, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), desc, k > 0);
+    const uint32_t off = ((k / 4) * kAttnTile * 128 + (k % 4) * 32) / 16;
+    mma_ss(d, a + off, b + off, desc, k > 0);
   }
 }
-// One product with a TMEM operand: 128 x D, contraction over the 128 rows of b.  The operand's two halves, written by
-// different warps, start HALF columns apart.
-template <int HALF>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
-  for (int k = 0; k < kAttnTile / 16; ++k)
-    mma_ts(d, a + (k / 4) * HALF + (k % 4) * 8, smem_desc(b + k * 2048, kAttnTile * 128, 1024), desc, add || k > 0);
+// With a TMEM operand: 128 x D, contraction over the 128 rows of b.  The operand's four parts, written by
+// different warps, start PART columns apart.
+template <int PART>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+#pragma unroll
+  for (int k = 0; k < kAttnTile / 16; ++k) mma_ts(d, a + (k / 2) * PART + (k % 2) * 8, b + k * 128, desc, add || k > 0);
 }
+// Descriptors of a tile read along its columns and along its rows.
+__device__ __forceinline__ uint64_t by_columns(uint32_t addr) { return smem_desc(addr, 16, 1024); }
+__device__ __forceinline__ uint64_t by_rows(uint32_t addr) { return smem_desc(addr, kAttnTile * 128, 1024); }
 
 // COLS fp32 columns of TMEM (from `col` on) as T, times f, into a staged tile of 128 rows.
 template <typename T, int COLS>
@@ -187,9 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_load_4d(dst + S::kTileBytes + c * kAttnTile * 128, &map_v, &bar.full[st], c * 64, (t0 + j) * kAttnTile, kv_head, b);
     }
   };
-  if (warp == 9) {
+  if (warp == kIssuer) {
     tmem_alloc(&tmem_slot, 512);
-  } else if (warp == 8) {  // the first copies are under way before the block meets
+  } else if (warp == kCopier) {  // the first copies are under way before the block meets
     if (elect_one()) {
       raised = 0;
       init_barriers(bar);
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Guard guard{&raised, bp.status};
   bool ok = true;
 
-  if (warp == 8) {
+  if (warp == kCopier) {
     if (n > 0 && elect_one()) {
       int j = min(n, S::kStages);
       for (; j < n; ++j) {
@@ -224,15 +235,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssuer) {
     if (n > 0) {
       constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
       constexpr uint32_t kRows = mma_desc<T>(128, D, false, true);
-      const uint32_t aq = smem_addr(sq), ado = smem_addr(sdo), akv = smem_addr(skv);
+      const uint64_t dq = by_columns(smem_addr(sq)), ddo = by_columns(smem_addr(sdo));
+      const uint64_t dkv = by_columns(smem_addr(skv)), dkv_rows = by_rows(smem_addr(skv));
       const uint4* dead = p.plan.kdead != nullptr ? p.plan.kdead + static_cast<int64_t>(b) * bp.nk + t0 : nullptr;
-      const bool leader = elect_one();
       ok = guard.wait_warp(&bar.fixed_full, 0);
-      auto stage = [&](int j) { return akv + (j % S::kStages) * 2 * S::kTileBytes; };
+      auto stage = [&](int j) { return static_cast<uint64_t>((j % S::kStages) * (2 * S::kTileBytes / 16)); };
       auto arrived = [&](int j) {  // K and V of tile j; padding keys cleared
         ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
         if (!ok) return;
@@ -246,15 +257,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto scores = [&](int j) {
-        if (leader) {
-          mma_scores<D>(tmem + kColS, aq, stage(j), kScores);
+        if (elect_one()) {
+          mma_scores<D>(tmem + kColS, dq, dkv + stage(j), kScores);
           mma_commit(&bar.s_full);
         }
         __syncwarp();
       };
       auto products = [&](int j) {
-        if (leader) {
-          mma_scores<D>(tmem + kColDP, ado, stage(j) + S::kTileBytes, kScores);
+        if (elect_one()) {
+          mma_scores<D>(tmem + kColDP, ddo, dkv + (stage(j) + S::kTileBytes / 16), kScores);
           mma_commit(&bar.dp_full);
         }
         __syncwarp();
@@ -275,15 +286,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = guard.wait_warp(&bar.ds_full, j & 1))) break;
         tc_fence_after();
         if (j + 1 < n) products(j + 1);
-        if (leader) {
-          mma_rows<32>(tmem + kColDQ, tmem + kColDS, stage(j), kRows, j > 0);
+        if (elect_one()) {
+          mma_rows<16>(tmem + kColDQ, tmem + kColDS, dkv_rows + stage(j), kRows, j > 0);
           mma_commit(&bar.empty[j % S::kStages]);
           mma_commit(&bar.second_done);
         }
         __syncwarp();
       }
       if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (leader) {
+        if (elect_one()) {
           mma_commit(&bar.drain);
           Guard::drain(&bar.drain, 0);
         }
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int r = (warp % 4) * 32 + lane, half = warp / 4;
+    const int r = (warp % 4) * 32 + lane, part = warp / 4;
     const int i = qt * kAttnTile + r;
     const bool valid = i < p.sq;
     const int2 range = valid ? attn_row_range(p, b, i) : make_int2(0, 0);
@@ -304,13 +315,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
     for (int j = 0; j < n; ++j) {
-      const int key0 = (t0 + j) * kAttnTile + half * kHalf;
-      const bool full = tr.z <= key0 && tr.w >= key0 + kHalf;
+      const int key0 = (t0 + j) * kAttnTile + part * kPart;
+      const bool full = tr.z <= key0 && tr.w >= key0 + kPart;
       if (!(ok = guard.wait_warp(&bar.s_full, j & 1))) break;
       tc_fence_after();
-      float pf[kHalf];  // scores, then probability times the cap's factor
-      tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
-      tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
+      float pf[kPart];  // scores, then probability times the cap's factor
+      tmem_ld32(lanes + kColS + part * kPart, reinterpret_cast<uint32_t*>(pf));
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(&bar.s_free);
@@ -318,16 +328,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!full) {
         const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
 #pragma unroll
-        for (int c = 0; c < kHalf; ++c) pf[c] = from + c < len ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
+        for (int c = 0; c < kPart; ++c) pf[c] = from + c < len ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
       }
       const float d0 = static_cast<float>(key0 - pos);
       // The distance's sign is known (masked pairs do not count): the bias joins the log-sum.
       const bool behind = MODE != kPlain &&
-                          __all_sync(0xffffffffu, key0 + kHalf - 1 <= pos || (p.causal && p.plan.range == nullptr));
+                          __all_sync(0xffffffffu, key0 + kPart - 1 <= pos || (p.causal && p.plan.range == nullptr));
       if (MODE == kPlain || behind || slope == 0.f) {
         const float base = fmaf(slope, d0, nlse);
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 2) {
+        for (int c = 0; c < kPart; c += 2) {
           const Pair x(pf[c], pf[c + 1]);
           const Pair add = MODE == kPlain ? nlse2 : Pair(fmaf(slope, static_cast<float>(c), base), fmaf(slope, static_cast<float>(c + 1), base));
           float e0, e1;
@@ -342,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < kHalf; ++c) {
+        for (int c = 0; c < kPart; ++c) {
           const float u = pf[c] * bp.sc.cap_inv, f = MODE == kCapped ? fmaf(-u, u, 1.f) : 1.f;
           const float x = fmaf(pf[c], MODE == kCapped ? 1.f : bp.sc.c, fmaf(-slope, fabsf(d0 + c), nlse));
           pf[c] = ex2(x) * (f * prob_unshift<T>());
@@ -350,11 +360,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
       tc_fence_after();
-      uint32_t w[32];
+      uint32_t w[kPart / 2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kPart / 32; ++c) {
         float dp[32];
-        tmem_ld32(lanes + kColDP + half * kHalf + c * 32, reinterpret_cast<uint32_t*>(dp));
+        tmem_ld32(lanes + kColDP + part * kPart + c * 32, reinterpret_cast<uint32_t*>(dp));
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -374,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
         tc_fence_after();
       }
-      tmem_st32(lanes + kColDS + half * 32, w);
+      tmem_st16(lanes + kColDS + part * 16, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar.ds_full);
@@ -398,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     store_tile<D>(&map_dq, sq, qt * kAttnTile, h, b);
     bulk_wait_read();
   }
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == kIssuer) tmem_free(tmem, 512);
 }
 
 // --- dk, dv -----------------------------------------------------------------------------------------------------
@@ -438,10 +448,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv,
                const __grid_constant__ BwdParams bp) {
   using S = Shape<D>;
-  // D = 64 leaves room for P and dS beside S and dP; else each half of the warps writes
-  // them over the scores that it alone has read.
+  // D = 64 leaves room for P and dS beside S and dP; else each warp writes them over
+  // the scores that it alone has read.
   constexpr bool kOwn = D == 64;
-  constexpr int kHalfCols = kOwn ? 32 : 64;
+  constexpr int kPartCols = kOwn ? 16 : 32;
   constexpr int kColS = 0, kColDP = 128, kColDV = 256, kColDK = 256 + D;
   constexpr int kColP = kOwn ? 384 : kColS, kColDS = kOwn ? 448 : kColDP;
   const AttnParams& p = bp.a;
@@ -463,9 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int key0 = id / p.b * kAttnTile;  // the first keys of a causal mask are seen by the most rows
   const int group = p.hq / p.hk;
 
-  if (warp == 9) {
+  if (warp == kIssuer) {
     tmem_alloc(&tmem_slot, 512);
-  } else if (warp == 8) {  // the first copies are under way before the block meets
+  } else if (warp == kCopier) {  // the first copies are under way before the block meets
     if (elect_one()) {
       raised = 0;
       first_tile = 0x7fffffff;
@@ -509,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const bool some = it.begin();
 
-  if (warp == 8) {
+  if (warp == kCopier) {
     if (some && elect_one()) {
       int j = 0;
       bool more = true;
@@ -534,14 +544,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!some || raised) Guard::drain(&bar.fixed_full, 0);
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssuer) {
     if (some) {
       constexpr uint32_t kScores = mma_desc<T>(128, 128, false, false);
       constexpr uint32_t kRows = mma_desc<T>(128, D, false, true);
-      const uint32_t ak = smem_addr(sk), av = smem_addr(sv), aqd = smem_addr(sqd);
-      const bool leader = elect_one();
+      const uint64_t dk = by_columns(smem_addr(sk)), dv = by_columns(smem_addr(sv));
+      const uint64_t dqd = by_columns(smem_addr(sqd)), dqd_rows = by_rows(smem_addr(sqd));
       ok = guard.wait_warp(&bar.fixed_full, 0);
-      auto stage = [&](int j) { return aqd + (j % S::kStages) * 2 * S::kTileBytes; };
+      auto stage = [&](int j) { return static_cast<uint64_t>((j % S::kStages) * (2 * S::kTileBytes / 16)); };
       auto arrived = [&](int j) {  // Q and dO of step j; rows without keys cleared
         ok = ok && guard.wait_warp(&bar.full[j % S::kStages], (j / S::kStages) & 1);
         if (!ok || it.full) return;
@@ -553,29 +563,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto scores = [&](int j) {
-        if (leader) {
-          mma_scores<D>(tmem + kColS, ak, stage(j), kScores);
+        if (elect_one()) {
+          mma_scores<D>(tmem + kColS, dk, dqd + stage(j), kScores);
           mma_commit(&bar.s_full);
         }
         __syncwarp();
       };
       auto products = [&](int j) {
-        if (leader) {
-          mma_scores<D>(tmem + kColDP, av, stage(j) + S::kTileBytes, kScores);
+        if (elect_one()) {
+          mma_scores<D>(tmem + kColDP, dv, dqd + (stage(j) + S::kTileBytes / 16), kScores);
           mma_commit(&bar.dp_full);
         }
         __syncwarp();
       };
       auto add_dv = [&](int j) {
-        if (leader) {
-          mma_rows<kHalfCols>(tmem + kColDV, tmem + kColP, stage(j) + S::kTileBytes, kRows, j > 0);
+        if (elect_one()) {
+          mma_rows<kPartCols>(tmem + kColDV, tmem + kColP, dqd_rows + (stage(j) + S::kTileBytes / 16), kRows, j > 0);
           mma_commit(&bar.first_done);
         }
         __syncwarp();
       };
       auto add_dk = [&](int j) {
-        if (leader) {
-          mma_rows<kHalfCols>(tmem + kColDK, tmem + kColDS, stage(j), kRows, j > 0);
+        if (elect_one()) {
+          mma_rows<kPartCols>(tmem + kColDK, tmem + kColDS, dqd_rows + stage(j), kRows, j > 0);
           mma_commit(&bar.empty[j % S::kStages]);
           mma_commit(&bar.second_done);
         }
@@ -620,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (leader) {
+        if (elect_one()) {
           mma_commit(&bar.drain);
           Guard::drain(&bar.drain, 0);
         }
@@ -628,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int r = (warp % 4) * 32 + lane, half = warp / 4;
+    const int r = (warp % 4) * 32 + lane, part = warp / 4;
     const int key = key0 + r;
     const Pair c2(bp.sc.c, bp.sc.c), inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
     const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
@@ -637,34 +647,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     int j = 0;
     for (; more; ++j) {
       const int st = j % S::kStages;
-      const float* stats = reinterpret_cast<const float*>(rows + st * S::kRowBytes) + half * kHalf;
-      const int2* range = reinterpret_cast<const int2*>(rows + st * S::kRowBytes + 1024) + half * kHalf;
-      const int row0 = it.t * kAttnTile + half * kHalf;
+      const float* stats = reinterpret_cast<const float*>(rows + st * S::kRowBytes) + part * kPart;
+      const int2* range = reinterpret_cast<const int2*>(rows + st * S::kRowBytes + 1024) + part * kPart;
+      const int row0 = it.t * kAttnTile + part * kPart;
       const bool full = it.full;
       const float slope = MODE != kPlain && p.slopes != nullptr ? p.slopes[hk * group + it.g] * kLog2e : 0.f;
       more = it.next();
       if (!(ok = guard.wait_warp(&bar.full[st], (j / S::kStages) & 1) && guard.wait_warp(&bar.s_full, j & 1))) break;
       tc_fence_after();
-      float pf[kHalf];  // scores, then probability times the cap's factor
-      tmem_ld32(lanes + kColS + half * kHalf, reinterpret_cast<uint32_t*>(pf));
-      tmem_ld32(lanes + kColS + half * kHalf + 32, reinterpret_cast<uint32_t*>(pf) + 32);
+      float pf[kPart];  // scores, then probability times the cap's factor
+      tmem_ld32(lanes + kColS + part * kPart, reinterpret_cast<uint32_t*>(pf));
       tmem_wait_ld();
       if (MODE == kCapped) cap_scores(pf, bp.sc);
       const int first_pos = row0 + p.sk - p.sq;
       if (!full) {
         if (p.plan.range != nullptr) {
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 2) {
+          for (int c = 0; c < kPart; c += 2) {
             const int4 v = *reinterpret_cast<const int4*>(range + c);
             pf[c] = key >= v.x && key < v.y ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
             pf[c + 1] = key >= v.z && key < v.w ? pf[c + 1] : (MODE == kCapped ? kMasked : -INFINITY);
           }
         } else if (p.causal) {  // rows from position `key` on
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) pf[c] = c >= key - first_pos ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
+          for (int c = 0; c < kPart; ++c) pf[c] = c >= key - first_pos ? pf[c] : (MODE == kCapped ? kMasked : -INFINITY);
         }
       }
-      uint32_t w[32];
+      uint32_t w[kPart / 2];
       // Distances are row - key here.  With a known sign (masked pairs do not count) they go two at a time.
       const float d0 = static_cast<float>(first_pos - key);
       const bool ahead = MODE != kPlain &&
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float base = prob_shift<T>() - slope * d0;
       const Pair shift2(prob_shift<T>(), prob_shift<T>());
 #pragma unroll
-      for (int c = 0; c < kHalf; c += 4) {
+      for (int c = 0; c < kPart; c += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(stats + c);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -705,16 +714,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = guard.wait_warp(&bar.first_done, (j - 1) & 1))) break;
         tc_fence_after();
       }
-      tmem_st32(lanes + kColP + half * kHalfCols, w);
+      tmem_st16(lanes + kColP + part * kPartCols, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar.p_full);
       if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kPart / 32; ++c) {
         float dp[32];
-        tmem_ld32(lanes + kColDP + half * kHalf + c * 32, reinterpret_cast<uint32_t*>(dp));
+        tmem_ld32(lanes + kColDP + part * kPart + c * 32, reinterpret_cast<uint32_t*>(dp));
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
@@ -734,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = guard.wait_warp(&bar.second_done, (j - 1) & 1))) break;
         tc_fence_after();
       }
-      tmem_st32(lanes + kColDS + half * kHalfCols, w);
+      tmem_st16(lanes + kColDS + part * kPartCols, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar.ds_full);
@@ -760,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     store_tile<D>(&map_dk, sk, key0, hk, b);
     bulk_wait_read();
   }
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == kIssuer) tmem_free(tmem, 512);
 }
 
 template <typename T, int D, Scores MODE>
