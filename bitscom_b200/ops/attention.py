@@ -24,7 +24,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _ext
 
@@ -100,22 +99,6 @@ def attention_mask(
                          None if prefix is None else prefix.clone())
 
 
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, plan, slopes, causal, scale, cap):
-        out, lse, lo = _ext._C.attention_forward(q, k, v, plan, slopes, causal, scale, cap, True)
-        ctx.save_for_backward(q, k, v, out, lse, lo, plan, slopes)
-        ctx.rest = (causal, scale, cap)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, lo, plan, slopes = ctx.saved_tensors
-        dq, dk, dv = _ext._C.attention_backward(dout, q, k, v, out, lse, lo, plan, slopes, *ctx.rest)
-        return dq, dk, dv, None, None, None, None, None
-
-
 def attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -179,7 +162,7 @@ def attention(
         raise ValueError("the mask was built from CPU tensors, q is on " + str(q.device))
     plan = None if mask is None else mask.plan
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, plan, slopes, causal, scale, cap)
+        return _ext._C.attention_train(q, k, v, plan, slopes, causal, scale, cap)
     return _ext._C.attention_forward(q, k, v, plan, slopes, causal, scale, cap, False)[0]
 
 

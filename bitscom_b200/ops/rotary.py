@@ -14,7 +14,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _ext
 
@@ -24,24 +23,6 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, device=None) -> torc
     if rotated < 2 or rotated % 2:
         raise ValueError(f"rotated must be a positive even number, got {rotated}")
     return base ** (-torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated)
-
-
-class _QkNormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, freq, wq, wk, positions, eps, interleaved):
-        ctx.save_for_backward(q, k, freq, wq, wk, positions)
-        ctx.rest = (eps, interleaved)
-        return _ext._C.rotary_forward(q, k, freq, wq, wk, positions, eps, interleaved)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, freq, wq, wk, positions = ctx.saved_tensors
-        want = ctx.needs_input_grad[3] or ctx.needs_input_grad[4]
-        dq, dk, dw = _ext._C.rotary_backward(gq, gk, q, k, freq, wq, wk, positions, *ctx.rest, want)
-        dwq = dw[0].to(wq.dtype) if ctx.needs_input_grad[3] else None
-        dwk = dw[1].to(wk.dtype) if ctx.needs_input_grad[4] else None
-        return dq, dk, None, dwq, dwk, None, None, None
 
 
 def qk_norm_rotary(
@@ -79,7 +60,7 @@ def qk_norm_rotary(
     if not _ext.use_cuda_kernels(q):
         return _qk_norm_rotary_cpu(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QkNormRotary.apply(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
+        return _ext._C.rotary_train(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
     return _ext._C.rotary_forward(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
 
 

@@ -29,8 +29,9 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const void* ids_base, in
                                                         int64_t ids_ss, const void* prefix, int prefix_bytes,
                                                         int causal, int sq, int sk, int nq, int nk, PlanView plan) {
   const int t = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  __shared__ long long id[kAttnTile + 1];
+  __shared__ long long id[kAttnTile];
   __shared__ int start[kAttnTile], end[kAttnTile];
+  __shared__ uint32_t begins[4];
   __shared__ int found;
   __shared__ int red[4][4];
   const bool docs = ids_base != nullptr;
@@ -53,15 +54,22 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const void* ids_base, in
   const int plen = static_cast<int>(p_len < 0 ? 0 : (p_len > sk ? sk : p_len));
 
   if (docs) {
-    if (tid < rows) id[tid] = first + tid >= 0 ? ids.at(first + tid) : -1;
+    if (tid < kAttnTile) id[tid] = tid < rows && first + tid >= 0 ? ids.at(first + tid) : -1;
+    __syncthreads();
+    if (tid < kAttnTile) {  // bit r: row r begins a run (row 0 counts as one, and so do the rows past the end)
+      const uint32_t m = __ballot_sync(0xffffffffu, tid == 0 || tid >= rows || id[tid] != id[tid - 1]);
+      if ((tid & 31) == 0) begins[tid >> 5] = m;
+    }
     __syncthreads();
     if (tid < rows) {
-      // Nearest changes of id inside the tile, by looking along it.
-      int a = tid, e = tid + 1;
-      while (a > 0 && id[a - 1] == id[tid] && first + a - 1 >= 0) --a;
-      while (e < rows && id[e] == id[tid]) ++e;
-      start[tid] = first + a;
-      end[tid] = first + e;
+      int w = tid >> 5;
+      uint32_t m = begins[w] & (0xffffffffu >> (31 - (tid & 31)));  // begins up to this row
+      while (m == 0u) m = begins[--w];
+      start[tid] = first + w * 32 + 31 - __clz(m);
+      w = tid >> 5;
+      m = (tid & 31) == 31 ? 0u : begins[w] & (0xffffffffu << ((tid & 31) + 1));  // begins behind it
+      while (m == 0u && ++w < 4) m = begins[w];
+      end[tid] = first + (m == 0u ? rows : min(rows, w * 32 + __ffs(m) - 1));
     }
     __syncthreads();
     // The first row's run to the left of the tile, and the last row's to the right.

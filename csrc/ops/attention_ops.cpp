@@ -371,6 +371,106 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rotary_backward(const at::Tensor&
   return {dq, dk, dw};
 }
 
+// ---------------------------------------------------------------------------
+// Autograd nodes, in C++: a training call of small tensors is bound by the host.
+// ---------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor or_undefined(const OptTensor& t) { return has(t) ? *t : at::Tensor(); }
+OptTensor if_defined(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// Passes gradients on that cannot be differentiated again: the operators have no second derivative.
+struct Once : public torch::autograd::Function<Once> {
+  static variable_list forward(AutogradContext*, variable_list grads_and_sources, int64_t grads) {
+    variable_list out;
+    for (int64_t i = 0; i < grads; ++i) out.push_back(grads_and_sources[i].defined() ? grads_and_sources[i].clone() : at::Tensor());
+    return out;
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "bitscom: the attention operators are differentiable once only");
+  }
+};
+
+variable_list once(variable_list grads, const variable_list& sources) {
+  if (!at::GradMode::is_enabled()) return grads;
+  const auto n = static_cast<int64_t>(grads.size());
+  variable_list all = std::move(grads);
+  for (auto& t : all)
+    if (!t.defined()) t = at::empty({0}, sources[0].options());
+  all.insert(all.end(), sources.begin(), sources.end());
+  return Once::apply(all, n);
+}
+
+struct Attention : public torch::autograd::Function<Attention> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const OptTensor& plan, const OptTensor& slopes, bool causal, double scale, double cap) {
+    auto [out, lse, lo] = attention_forward(q, k, v, plan, slopes, causal, scale, cap, true);
+    ctx->save_for_backward({q, k, v, out, lse, lo, or_undefined(plan), or_undefined(slopes)});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["cap"] = cap;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    variable_list d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dq, dk, dv] = attention_backward(g[0], s[0], s[1], s[2], s[3], s[4], if_defined(s[5]), if_defined(s[6]),
+                                             if_defined(s[7]), ctx->saved_data["causal"].toBool(),
+                                             ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble());
+      d = {dq, dk, dv};
+    }
+    d = once(std::move(d), {s[0], s[1], s[2], g[0]});
+    return {d[0], d[1], d[2], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor attention_train(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
+                           const OptTensor& slopes, bool causal, double scale, double cap) {
+  return Attention::apply(q, k, v, plan, slopes, causal, scale, cap);
+}
+
+struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
+                               const OptTensor& wq, const OptTensor& wk, const OptTensor& positions, double eps,
+                               bool interleaved) {
+    auto [oq, ok] = rotary_forward(q, k, freq, wq, wk, positions, eps, interleaved);
+    ctx->save_for_backward({q, k, freq, or_undefined(wq), or_undefined(wk), or_undefined(positions)});
+    ctx->saved_data["want_q"] = has(wq) && wq->requires_grad();
+    ctx->saved_data["want_k"] = has(wk) && wk->requires_grad();
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {oq, ok};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool want_q = ctx->saved_data["want_q"].toBool(), want_k = ctx->saved_data["want_k"].toBool();
+    variable_list d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dq, dk, dw] = rotary_backward(g[0], g[1], s[0], s[1], s[2], if_defined(s[3]), if_defined(s[4]),
+                                          if_defined(s[5]), ctx->saved_data["eps"].toDouble(),
+                                          ctx->saved_data["interleaved"].toBool(), want_q || want_k);
+      d = {dq, dk, want_q ? dw.select(0, 0).to(s[3].scalar_type()) : at::Tensor(),
+           want_k ? dw.select(0, 1).to(s[4].scalar_type()) : at::Tensor()};
+    }
+    variable_list sources = {s[0], s[1], g[0], g[1]};
+    for (const auto& w : {s[3], s[4]})
+      if (w.defined()) sources.push_back(w);
+    const variable_list r = once(d, sources);
+    return {r[0], r[1], at::Tensor(), want_q ? r[2] : at::Tensor(), want_k ? r[3] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_train(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
+                                                const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
+                                                double eps, bool interleaved) {
+  auto out = QkNormRotary::apply(q, k, freq, wq, wk, positions, eps, interleaved);
+  return {out[0], out[1]};
+}
+
 }  // namespace
 
 void register_attention_bindings(pybind11::module_& m) {
@@ -379,15 +479,14 @@ void register_attention_bindings(pybind11::module_& m) {
         py::arg("q_len"), py::arg("k_len"));
   m.def("attention_forward", &attention_forward, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"),
         py::arg("slopes"), py::arg("causal"), py::arg("scale"), py::arg("cap"), py::arg("want_lse"));
-  m.def("attention_backward", &attention_backward, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("out"), py::arg("lse"), py::arg("lo"), py::arg("plan"), py::arg("slopes"), py::arg("causal"), py::arg("scale"),
-        py::arg("cap"));
+  m.def("attention_train", &attention_train, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("slopes"),
+        py::arg("causal"), py::arg("scale"), py::arg("cap"));
   m.def("attention_status", [](bool reset) { return launch::attention_status(reset); }, py::arg("reset") = false,
         "1 once a wait of a tensor-core attention kernel on the current device ran out, else 0 (waits for the device).");
   m.def("rotary_forward", &rotary_forward, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
         py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
-  m.def("rotary_backward", &rotary_backward, py::arg("gq"), py::arg("gk"), py::arg("q"), py::arg("k"), py::arg("freq"),
-        py::arg("wq"), py::arg("wk"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"), py::arg("want_dw"));
+  m.def("rotary_train", &rotary_train, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
+        py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
 }
 
 }  // namespace bitscom_b200
