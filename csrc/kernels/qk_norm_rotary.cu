@@ -12,12 +12,19 @@
 // shuffle more.  When a half is not a whole number of pieces, the partners are
 // exchanged through shared memory.  Norms, rotations and sums are in fp32, with
 // one rounding at the end; the angle is formed and reduced to one turn in fp64
-// (a position of 10^6 times a frequency leaves fp32 five digits short), once
-// for each token and frequency and then shared by all heads of the token.
+// (a position of 10^6 times a frequency leaves fp32 five digits short).
 //
-// The gains' gradients are summed in registers over a block's heads, then over
-// the block's groups and over the blocks in a fixed order: no atomics, the same
-// bits every time.
+// A lane group takes a token, forms the angles of its own values once (4 % of the
+// time at 20 heads) and goes through the heads with them in registers, the next
+// heads' loads under way.  No lane group waits for another: with angles
+// formed by the block in shared memory and a head to a lane group, the barriers and the
+// divisions for each head held 131072 tokens x 20 heads x 128 (fp16) at 629 us; this
+// form takes 327 us (4.1 TB/s, 62 % of a copy).  Two blocks of 128
+// registers a thread an SM: three of 80 spill (452 us).
+//
+// The gains' gradients are summed in registers over a lane group's heads, then
+// over the block's groups and over the blocks in a fixed order: no atomics, the
+// same bits every time.
 #include <cuda_runtime.h>
 
 #include "attention_common.cuh"
@@ -28,23 +35,31 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kV = 8;  // values of a lane
+constexpr int kBlocks = 2;  // resident on an SM
+
+// A lane's 8 values as they lie in memory.
+template <typename T>
+struct Raw {
+  uint4 w[sizeof(T) / 2];
+};
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int count, float (&o)[kV]) {
+__device__ __forceinline__ void load8(const T* p, bool vec, int count, Raw<T>& o) {
   if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int i = 0; i < kV; ++i) o[i] = to_f32<T>(t[i]);
-    }
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) o.w[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
+    T* t = reinterpret_cast<T*>(o.w);
 #pragma unroll
-    for (int i = 0; i < kV; ++i) o[i] = i < count ? to_f32<T>(p[i]) : 0.f;
+    for (int i = 0; i < kV; ++i) t[i] = i < count ? p[i] : from_f32<T>(0.f);
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void values(const Raw<T>& r, bool live, float (&o)[kV]) {
+  const T* t = reinterpret_cast<const T*>(r.w);
+#pragma unroll
+  for (int i = 0; i < kV; ++i) o[i] = live ? to_f32<T>(t[i]) : 0.f;
 }
 
 template <typename T>
@@ -67,43 +82,28 @@ __device__ __forceinline__ void store8(T* p, bool vec, int count, const float (&
   }
 }
 
-// One head as a lane group holds it.
-struct Head {
-  unsigned b, i;  // batch entry and place in the row
-  int h;
-  bool key;
-};
-
-template <typename T>
-__device__ __forceinline__ T* at(const RotaryTensor& x, const Head& r, int col) {
-  return static_cast<T*>(x.ptr) + r.b * x.sb + r.i * x.ss + r.h * x.sh + col;
+template <int LANES, int U>
+__device__ __forceinline__ void group_sums(float (&v)[U]) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
 }
 
-// Rotates the lane's 8 values of a head.  `angles`: this token's (cos, sin).
-// SHUFFLE: the partner of every value lies at the same place of another lane.
+// Rotates the lane's 8 values of a head.  `cs`, `sn`: cosine and signed sine of each value's pair (1, 0 where
+// nothing is rotated): y cs + partner sn.
 template <int LANES, bool SHUFFLE>
-__device__ __forceinline__ void rotate(float (&y)[kV], const RotaryParams& p, const float2* angles, float sign, int lane,
-                                       float* exchange) {
-  const int r = p.rotated, half = r / 2, col = lane * kV;
+__device__ __forceinline__ void rotate(float (&y)[kV], const RotaryParams& p, const float (&cs)[kV], const float (&sn)[kV],
+                                       int from, int lane, float* exchange) {
+  float o[kV];
   if (p.interleaved) {  // neighbours: both in this lane
 #pragma unroll
-    for (int i = 0; i < kV; i += 2) {
-      if (col + i < r) {
-        const float2 a = angles[(col + i) / 2];
-        const float u = y[i], v = y[i + 1], sn = sign * a.y;
-        y[i] = u * a.x - v * sn;
-        y[i + 1] = v * a.x + u * sn;
-      }
-    }
-    return;
-  }
-  float o[kV];
-  if (SHUFFLE) {
-    const int step = half / kV;
-    const int from = lane < step ? lane + step : (lane < 2 * step ? lane - step : lane);
+    for (int i = 0; i < kV; ++i) o[i] = y[i ^ 1];
+  } else if (SHUFFLE) {
 #pragma unroll
     for (int i = 0; i < kV; ++i) o[i] = __shfl_sync(0xffffffffu, y[i], from, LANES);
   } else {
+    const int half = p.rotated / 2, col = lane * kV;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kV; ++i) exchange[col + i] = y[i];
@@ -111,128 +111,188 @@ __device__ __forceinline__ void rotate(float (&y)[kV], const RotaryParams& p, co
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
       const int c = col + i;
-      o[i] = c < half ? exchange[c + half] : (c < r ? exchange[c - half] : 0.f);
+      o[i] = c < half ? exchange[c + half] : (c < p.rotated ? exchange[c - half] : 0.f);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kV; ++i) {
-    const int c = col + i;
-    if (c < r) {
-      const bool low = c < half;
-      const float2 a = angles[low ? c : c - half];
-      y[i] = y[i] * a.x + (low ? -sign : sign) * a.y * o[i];
-    }
-  }
+  for (int i = 0; i < kV; ++i) y[i] = y[i] * cs[i] + sn[i] * o[i];
 }
 
-template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// What a lane keeps while it goes through the heads of one token.
+template <typename T>
+struct Lane {
+  int col, count, from, lane;
+  bool holds, vec;
+  float inv_d;
+  float cs[kV], sn[kV];
+  float* exchange;
+};
 
-// GRAD: dx and the gains' gradients.  A block takes `chunk` tokens at a time.
+// `n` heads of one tensor; AHEAD of them are on their way while one is worked on, which is what
+// keeps enough bytes in flight.  `rounds` is the most heads that any lane group of the warp has.
 template <typename T, int LANES, bool SHUFFLE, bool GRAD>
-__global__ void __launch_bounds__(kThreads) qk_kernel(const RotaryParams p, int chunk, bool vec) {
-  extern __shared__ float2 angles[];  // [chunk][rotated / 2]
-  __shared__ float exchange[SHUFFLE ? 1 : kThreads * kV];
-  __shared__ float gains[2][launch::kRotaryMaxDim];
-  constexpr int kGroups = kThreads / LANES;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int col = lane * kV, count = min(kV, p.d - col), half = p.rotated / 2;
-  const bool holds = col < p.d;
-  const float inv_d = 1.f / p.d;
-  const int heads = p.q.h + p.k.h;
-  for (int i = threadIdx.x; i < 2 * p.d; i += kThreads) {
-    const float* w = i < p.d ? p.wq : p.wk;
-    gains[i / p.d][i % p.d] = w != nullptr ? w[i % p.d] : 1.f;
-  }
-  float dw[2][kV];
+__device__ __forceinline__ void heads(const RotaryParams& p, const Lane<T>& ln, const T* in, int64_t in_sh, const T* grad,
+                                      int64_t grad_sh, T* out, int64_t out_sh, int n, int rounds, const float (&w)[kV],
+                                      float (&dw)[kV]) {
+  constexpr int AHEAD = sizeof(T) == 4 || GRAD ? 2 : 4, U = GRAD ? 1 : 2;
+  Raw<T> xr[AHEAD], gr[GRAD ? AHEAD : 1];
+  if (!ln.holds) n = 0;
 #pragma unroll
-  for (int i = 0; i < kV; ++i) dw[0][i] = dw[1][i] = 0.f;
-
-  // Token counts stay below 2^31 (checked by the caller): 32-bit divisions.
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * chunk; t0 < p.tokens; t0 += static_cast<int64_t>(gridDim.x) * chunk) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(chunk), p.tokens - t0));
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * half; i += kThreads) {
-      const unsigned t = static_cast<unsigned>(t0) + i / half;
-      int64_t pos = t % p.s;
-      if (p.positions != nullptr) {
-        const int64_t e = t / p.s * p.pos_sb + pos * p.pos_ss;
-        pos = p.pos_bytes == 8 ? static_cast<const long long*>(p.positions)[e] : static_cast<const int*>(p.positions)[e];
-      }
-      const double a = static_cast<double>(pos) * p.freq[i % half];
-      const double turns = rint(a * 0.15915494309189535);  // 1 / (2 pi)
-      const float x = static_cast<float>(fma(turns, -6.283185307179586, a) - turns * 2.4492935982947064e-16);
-      float sn, cs;
-      sincosf(x, &sn, &cs);
-      angles[i] = make_float2(cs, sn);
+  for (int u = 0; u < AHEAD; ++u) {
+    if (u < n) {
+      load8<T>(in + u * in_sh, ln.vec, ln.count, xr[u]);
+      if (GRAD) load8<T>(grad + u * grad_sh, ln.vec, ln.count, gr[u]);
     }
-    __syncthreads();
-    const int total = n * heads;
-    for (int r0 = 0; r0 < total; r0 += kGroups) {
-      const int row = r0 + group;
-      const bool live = row < total && holds;
-      Head hd;
-      const int in_chunk = min(row, total - 1) / heads;
-      hd.b = static_cast<unsigned>(t0 + in_chunk) / p.s;
-      hd.i = static_cast<unsigned>(t0 + in_chunk) % p.s;
-      hd.h = min(row, total - 1) % heads;
-      hd.key = hd.h >= p.q.h;
-      if (hd.key) hd.h -= p.q.h;
-      float x[kV], w[kV];
+  }
+  for (int h0 = 0; h0 < rounds; h0 += AHEAD) {
 #pragma unroll
-      for (int i = 0; i < kV; ++i) x[i] = w[i] = 0.f;
-      float g[kV];
-      if (live) {
-        load8<T>(at<T>(hd.key ? p.k : p.q, hd, col), vec, count, x);
-        if (GRAD) load8<T>(at<T>(hd.key ? p.gk : p.gq, hd, col), vec, count, g);
+    for (int a = 0; a < AHEAD; a += U) {  // U heads side by side: their chains of shuffles overlap
+      const int h = h0 + a;
+      float x[U][kV], g[U][kV], sum[U];
 #pragma unroll
-        for (int i = 0; i < kV; ++i) w[i] = i < count ? gains[hd.key][col + i] : 0.f;
-      } else if (GRAD) {
+      for (int u = 0; u < U; ++u) {
+        values<T>(xr[a + u], h + u < n, x[u]);
+        if (GRAD) values<T>(gr[GRAD ? a + u : 0], h + u < n, g[u]);
+        if (h + u + AHEAD < n) {
+          load8<T>(in + (h + u + AHEAD) * in_sh, ln.vec, ln.count, xr[a + u]);
+          if (GRAD) load8<T>(grad + (h + u + AHEAD) * grad_sh, ln.vec, ln.count, gr[GRAD ? a + u : 0]);
+        }
+        sum[u] = 0.f;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) g[i] = 0.f;
+        for (int i = 0; i < kV; ++i) sum[u] += x[u][i] * x[u][i];
       }
-      float sum = 0.f;
+      group_sums<LANES, U>(sum);
 #pragma unroll
-      for (int i = 0; i < kV; ++i) sum += x[i] * x[i];
-      const float rs = rsqrtf(group_sum<LANES>(sum) * inv_d + p.eps);
-      const float2* an = angles + in_chunk * half;
-      float* ex = SHUFFLE ? nullptr : exchange + group * LANES * kV;
+      for (int u = 0; u < U; ++u) {
+        const float rs = rsqrtf(sum[u] * ln.inv_d + p.eps);
+        sum[u] = rs;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) x[u][i] *= GRAD ? rs : rs * w[i];
+      }
       if (!GRAD) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) x[i] *= rs * w[i];
-        rotate<LANES, SHUFFLE>(x, p, an, 1.f, lane, ex);
-        if (live) store8<T>(at<T>(hd.key ? p.ok : p.oq, hd, col), vec, count, x);
+        for (int u = 0; u < U; ++u) rotate<LANES, SHUFFLE>(x[u], p, ln.cs, ln.sn, ln.from, ln.lane, ln.exchange);
       } else {
-        rotate<LANES, SHUFFLE>(g, p, an, -1.f, lane, ex);
-        float dot = 0.f;
+        float dot[U];
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          x[i] *= rs;  // n
-          const float gn = live ? g[i] * x[i] : 0.f;
-          if (hd.key)
-            dw[1][i] += gn;
-          else
-            dw[0][i] += gn;
-          dot += gn * w[i];
-          g[i] *= w[i];
+        for (int u = 0; u < U; ++u) {
+          rotate<LANES, SHUFFLE>(g[u], p, ln.cs, ln.sn, ln.from, ln.lane, ln.exchange);
+          dot[u] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kV; ++i) {
+            dw[i] += g[u][i] * x[u][i];
+            g[u][i] *= w[i];
+            dot[u] += g[u][i] * x[u][i];
+          }
         }
-        dot = group_sum<LANES>(dot) * inv_d;
+        group_sums<LANES, U>(dot);
 #pragma unroll
-        for (int i = 0; i < kV; ++i) x[i] = rs * (g[i] - x[i] * dot);
-        if (live) store8<T>(at<T>(hd.key ? p.ok : p.oq, hd, col), vec, count, x);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < kV; ++i) x[u][i] = sum[u] * (g[u][i] - x[u][i] * (dot[u] * ln.inv_d));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (h + u < n) store8<T>(out + (h + u) * out_sh, ln.vec, ln.count, x[u]);
+    }
+  }
+}
+
+// Cosine and sine of position * frequency.
+__device__ __forceinline__ void turn(int64_t pos, double freq, float* cs, float* sn) {
+  const double a = static_cast<double>(pos) * freq;
+  const double turns = rint(a * 0.15915494309189535);  // 1 / (2 pi)
+  sincosf(static_cast<float>(fma(turns, -6.283185307179586, a) - turns * 2.4492935982947064e-16), sn, cs);
+}
+
+// GRAD: dx and the gains' gradients.  A lane group takes a token (or one of `split` parts of its heads), forms the
+// angles of its values and goes through the heads with them in registers; nothing is shared between groups.
+template <typename T, int LANES, bool SHUFFLE, bool GRAD>
+__global__ void __launch_bounds__(kThreads, kBlocks) qk_kernel(const RotaryParams p, int split, bool vec) {
+  constexpr int kGroups = kThreads / LANES;
+  __shared__ float exchange[SHUFFLE ? 1 : kThreads * kV];
+  const int group = threadIdx.x / LANES;
+  const int half = p.rotated / 2, all = p.q.h + p.k.h;
+  const int per = (all + split - 1) / split;
+  Lane<T> ln;
+  ln.lane = threadIdx.x % LANES;
+  ln.col = ln.lane * kV;
+  ln.count = min(kV, p.d - ln.col);
+  ln.holds = ln.col < p.d;
+  ln.vec = vec;
+  ln.inv_d = 1.f / p.d;
+  ln.exchange = SHUFFLE ? nullptr : exchange + group * LANES * kV;
+  const int step = half / kV;
+  ln.from = ln.lane < step ? ln.lane + step : (ln.lane < 2 * step ? ln.lane - step : ln.lane);
+  float wq[kV], wk[kV], dwq[kV], dwk[kV];
+#pragma unroll
+  for (int i = 0; i < kV; ++i) {
+    wq[i] = wk[i] = i < ln.count ? 1.f : 0.f;
+    if (i < ln.count && p.wq != nullptr) wq[i] = p.wq[ln.col + i];
+    if (i < ln.count && p.wk != nullptr) wk[i] = p.wk[ln.col + i];
+    dwq[i] = dwk[i] = 0.f;
+  }
+
+  // All lanes of a warp make the same number of steps (the shuffles want them); token
+  // counts stay below 2^31 (checked by the caller): 32-bit divisions.
+  const int64_t items = p.tokens * split, stride = static_cast<int64_t>(gridDim.x) * kGroups;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group / (32 / LANES) * (32 / LANES); first < items; first += stride) {
+    const int64_t item = first + group % (32 / LANES);
+    const bool has = item < items;
+    const unsigned t = has ? static_cast<unsigned>(split == 1 ? item : item / split) : 0u;
+    const int part = split == 1 ? 0 : static_cast<int>(item % split);
+    const unsigned b = t / p.s, i0 = t % p.s;
+    int64_t pos = i0;
+    if (p.positions != nullptr) {
+      const int64_t e = b * p.pos_sb + i0 * p.pos_ss;
+      pos = p.pos_bytes == 8 ? static_cast<const long long*>(p.positions)[e] : static_cast<const int*>(p.positions)[e];
+    }
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < kV; i += 2) {
+        ln.cs[i] = ln.cs[i + 1] = 1.f;
+        ln.sn[i] = ln.sn[i + 1] = 0.f;
+        if (ln.col + i < p.rotated) {
+          turn(pos, p.freq[(ln.col + i) / 2], &ln.cs[i], &ln.sn[i + 1]);
+          ln.cs[i + 1] = ln.cs[i];
+          ln.sn[i] = -ln.sn[i + 1];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const int c = ln.col + i;
+        ln.cs[i] = 1.f;
+        ln.sn[i] = 0.f;
+        if (c < p.rotated) {
+          turn(pos, p.freq[c < half ? c : c - half], &ln.cs[i], &ln.sn[i]);
+          if (c < half) ln.sn[i] = -ln.sn[i];
+        }
       }
     }
+    if (GRAD) {
+#pragma unroll
+      for (int i = 0; i < kV; ++i) ln.sn[i] = -ln.sn[i];
+    }
+    const auto at = [&](const RotaryTensor& x, int h) {
+      return static_cast<T*>(x.ptr) + b * x.sb + i0 * x.ss + h * x.sh + ln.col;
+    };
+    // Heads [h0, h1) of the list q heads, k heads.
+    const int h0 = min(all, part * per), h1 = min(all, h0 + per);
+    const int q0 = min(h0, p.q.h), q1 = min(h1, p.q.h), k0 = max(h0, p.q.h) - p.q.h, k1 = max(h1, p.q.h) - p.q.h;
+    const int nq = has ? q1 - q0 : 0, nk = has ? k1 - k0 : 0;
+    const int rounds_q = __reduce_max_sync(0xffffffffu, nq), rounds_k = __reduce_max_sync(0xffffffffu, nk);
+    heads<T, LANES, SHUFFLE, GRAD>(p, ln, at(p.q, q0), p.q.sh, GRAD ? at(p.gq, q0) : nullptr, p.gq.sh, at(p.oq, q0),
+                                      p.oq.sh, nq, rounds_q, wq, dwq);
+    heads<T, LANES, SHUFFLE, GRAD>(p, ln, at(p.k, k0), p.k.sh, GRAD ? at(p.gk, k0) : nullptr, p.gk.sh, at(p.ok, k0),
+                                      p.ok.sh, nk, rounds_k, wk, dwk);
   }
   if (GRAD && p.partial != nullptr) {
     __shared__ float sums[kThreads * kV];
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kV; ++i) sums[group * LANES * kV + col + i] = which ? dw[1][i] : dw[0][i];
+      for (int i = 0; i < kV; ++i) sums[group * LANES * kV + ln.col + i] = which ? dwk[i] : dwq[i];
       __syncthreads();
       for (int c = threadIdx.x; c < p.d; c += kThreads) {
         float v = 0.f;
@@ -264,16 +324,14 @@ bool aligned(const RotaryTensor& x, int size) {
   return reinterpret_cast<uintptr_t>(x.ptr) % 16 == 0 && x.sb % m == 0 && x.ss % m == 0 && x.sh % m == 0;
 }
 
-// Tokens of a chunk: enough heads for every lane group to take four, while
-// there are blocks for all SMs.
-int chunk_tokens(const RotaryParams& p, int sms) {
+// Parts of a token's heads: one, so that angles are formed once for all heads, unless the
+// tokens are too few to fill every SM's blocks twice.
+int head_split(const RotaryParams& p, int sms) {
   const int lanes = p.d <= 64 ? 8 : (p.d <= 128 ? 16 : 32);
-  const int heads = p.q.h + p.k.h, groups = kThreads / lanes;
-  int64_t n = (4 * groups + heads - 1) / heads;
-  const int64_t most = (p.tokens + 2 * sms - 1) / (2 * sms);
-  if (n > most) n = most;
-  if (n > 32) n = 32;
-  return static_cast<int>(n < 1 ? 1 : n);
+  const int groups = kThreads / lanes, all = p.q.h + p.k.h;
+  int split = 1;
+  while (split < groups && 4 * split <= 2 * all && p.tokens * split < int64_t(2) * kBlocks * sms * groups) split *= 2;
+  return split;
 }
 
 template <typename T, int LANES, bool SHUFFLE, bool GRAD>
@@ -281,11 +339,9 @@ void run(const RotaryParams& p, int sms, cudaStream_t s) {
   const int size = sizeof(T);
   const bool vec = p.d % kV == 0 && aligned(p.q, size) && aligned(p.k, size) && aligned(p.oq, size) &&
                    aligned(p.ok, size) && aligned(p.gq, size) && aligned(p.gk, size);
-  const int chunk = chunk_tokens(p, sms);
-  int64_t blocks = (p.tokens + chunk - 1) / chunk;
-  if (GRAD) blocks = launch::qk_norm_rotary_blocks(p, sms);
-  const size_t bytes = sizeof(float2) * chunk * (p.rotated / 2);
-  qk_kernel<T, LANES, SHUFFLE, GRAD><<<static_cast<unsigned>(blocks), kThreads, bytes, s>>>(p, chunk, vec);
+  const int split = head_split(p, sms), groups = kThreads / LANES;
+  const int64_t blocks = GRAD ? launch::qk_norm_rotary_blocks(p, sms) : (p.tokens * split + groups - 1) / groups;
+  qk_kernel<T, LANES, SHUFFLE, GRAD><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(p, split, vec);
 }
 
 template <typename T, bool GRAD>
@@ -314,9 +370,9 @@ void by_type(const RotaryParams& p, int sms, cudaStream_t s) {
 namespace launch {
 
 int qk_norm_rotary_blocks(const RotaryParams& p, int sms) {
-  const int chunk = chunk_tokens(p, sms);
-  const int64_t all = (p.tokens + chunk - 1) / chunk;
-  return static_cast<int>(all < 4 * sms ? all : 4 * sms);  // four resident blocks an SM, then further chunks each
+  const int groups = kThreads / (p.d <= 64 ? 8 : (p.d <= 128 ? 16 : 32));
+  const int64_t all = (p.tokens * head_split(p, sms) + groups - 1) / groups;
+  return static_cast<int>(all < kBlocks * sms ? all : kBlocks * sms);  // the resident blocks, further tokens in turn
 }
 
 void qk_norm_rotary_forward(const RotaryParams& p, int sms, cudaStream_t s) { by_type<false>(p, sms, s); }
