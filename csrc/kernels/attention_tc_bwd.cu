@@ -1,7 +1,7 @@
 // Masked attention backward on the 5th-generation tensor cores.
 //
-//   stats:  -log2 sum and delta = dout.(o + what its rounding took), for both kernels below
-//   dq:     a CTA holds 128 rows of Q and dO and walks over their keys:
+//   dq:     a CTA holds 128 rows of Q and dO, forms delta = dout.(o + what its rounding took) for
+//           itself and the next kernel, and walks over the rows' keys:
 //             S = Q K^T, dP = dO V^T, dS = P (dP - delta), dQ += dS K
 //   dk, dv: a CTA holds 128 keys and values and walks over the rows that see them, through all
 //           query heads that share the key head:
@@ -124,42 +124,6 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* m, const char* til
   bulk_commit();
 }
 
-// --- row statistics ---------------------------------------------------------------------------------------------
-
-// LANES lanes a row, 16 bytes each.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(256) stats_kernel(const BwdParams bp) {
-  const AttnParams& p = bp.a;
-  constexpr int kRowsPerBlock = 256 / LANES;
-  const int64_t padded = static_cast<int64_t>(bp.nq) * kAttnTile;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / LANES;
-  if (row >= padded * p.b * p.hq) return;  // whole lane groups: padded is a multiple of them
-  const int i = static_cast<int>(row % padded);
-  const int h = static_cast<int>(row / padded % p.hq), b = static_cast<int>(row / padded / p.hq);
-  const int col = threadIdx.x % LANES * 8;
-  float sum = 0.f, lse = INFINITY;
-  if (i < p.sq) {
-    lse = p.lse[(static_cast<int64_t>(b) * p.hq + h) * p.sq + i];
-    if (col < p.d) {
-      const int64_t at = b * p.o.sb + h * p.o.sh + i * p.o.ss + col;
-      const uint4 uo = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.o.ptr) + at);
-      const uint4 ul = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo.ptr) + at);
-      const uint4 ug = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + b * p.dout.sb +
-                                                       h * p.dout.sh + i * p.dout.ss + col);
-      const T *o = reinterpret_cast<const T*>(&uo), *l = reinterpret_cast<const T*>(&ul), *g = reinterpret_cast<const T*>(&ug);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += (to_f32<T>(o[e]) + to_f32<T>(l[e])) * to_f32<T>(g[e]);
-    }
-  }
-#pragma unroll
-  for (int x = LANES / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-  if (threadIdx.x % LANES == 0) {
-    float* s = p.stats + (row / kAttnTile) * 2 * kAttnTile + row % kAttnTile;
-    s[0] = -lse;
-    s[kAttnTile] = lse == INFINITY ? 0.f : sum;  // a row without keys: whatever its gradient holds
-  }
-}
-
 // --- dq ---------------------------------------------------------------------------------------------------------
 
 template <typename T, int D, Scores MODE>
@@ -174,6 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int raised;
+  __shared__ float partial[4][kAttnTile];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* sq = base;
   char* sdo = base + S::kTileBytes;
@@ -308,8 +273,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int2 range = valid ? attn_row_range(p, b, i) : make_int2(0, 0);
     const int pos = i + p.sk - p.sq;
     const float slope = MODE != kPlain && p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
-    const float* st = p.stats + ((static_cast<int64_t>(b) * p.hq + h) * bp.nq + qt) * 2 * kAttnTile + r;
-    const float nlse = st[0] + prob_shift<T>(), delta = st[kAttnTile];
+    // delta = dout . (o + what its rounding took), a quarter of the columns a thread; kept for the other kernel.
+    float sum = 0.f, lse = INFINITY;
+    if (valid) {
+      lse = p.lse[(static_cast<int64_t>(b) * p.hq + h) * p.sq + i];
+      const int64_t at = b * p.o.sb + h * p.o.sh + i * p.o.ss, at_g = b * p.dout.sb + h * p.dout.sh + i * p.dout.ss;
+#pragma unroll
+      for (int c = part * (D / 4); c < (part + 1) * (D / 4); c += 8) {
+        if (c >= p.d) continue;
+        const uint4 uo = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.o.ptr) + at + c);
+        const uint4 ul = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.lo.ptr) + at + c);
+        const uint4 ug = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + at_g + c);
+        const T *o = reinterpret_cast<const T*>(&uo), *l = reinterpret_cast<const T*>(&ul), *g = reinterpret_cast<const T*>(&ug);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += (to_f32<T>(o[e]) + to_f32<T>(l[e])) * to_f32<T>(g[e]);
+      }
+    }
+    partial[part][r] = sum;
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    static_assert(kCompute == 512, "threads of the barrier");
+    // A row without keys: whatever its gradient holds.
+    const float delta = lse == INFINITY ? 0.f : (partial[0][r] + partial[1][r]) + (partial[2][r] + partial[3][r]);
+    if (part == 0) {
+      float* st = p.stats + ((static_cast<int64_t>(b) * p.hq + h) * bp.nq + qt) * 2 * kAttnTile + r;
+      st[0] = -lse;
+      st[kAttnTile] = delta;
+    }
+    const float nlse = prob_shift<T>() - lse;
     const Pair nlse2(nlse, nlse), delta2(-delta, -delta), c2(bp.sc.c, bp.sc.c);
     const Pair inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
     const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
@@ -780,9 +770,6 @@ cudaError_t run(const BwdParams& bp, cudaStream_t s) {
       !attn_map(&k, p.k, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&v, p.v, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&dq, p.dq, p, p.hq, p.sq, kAttnTile, 1) ||
       !attn_map(&dk, p.dk, p, p.hk, p.sk, kAttnTile, 1) || !attn_map(&dv, p.dv, p, p.hk, p.sk, kAttnTile, 1))
     return cudaErrorInvalidValue;
-  constexpr int kLanes = D / 8, kRowsPerBlock = 256 / kLanes;
-  const int64_t rows = static_cast<int64_t>(bp.nq) * kAttnTile * p.b * p.hq;
-  stats_kernel<T, kLanes><<<static_cast<unsigned>((rows + kRowsPerBlock - 1) / kRowsPerBlock), 256, 0, s>>>(bp);
   cudaError_t e = cudaFuncSetAttribute(dq_kernel<T, D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(dkv_kernel<T, D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
