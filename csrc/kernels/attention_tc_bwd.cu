@@ -22,6 +22,12 @@
 // The MMAs of the next tile's S and dP are issued as soon as the arithmetic has read
 // (or, where P and dS share their columns, the second product has read) the present
 // ones, so that exponentials and products run side by side.
+//
+// Measured, 16 heads x 4096 rows, causal, both kernels: D = 64 194 us (with 8 warps of
+// arithmetic and half the columns a thread 215), D = 128 275 us, capped 339 us.  Of a step of
+// the dk/dv kernel (D = 64, 8 warps, 3300 clocks) 1700 went into exponentials and 700 into
+// dS, the MMAs waiting: the arithmetic's latency bounds it, then 1500 (D = 64) to 2900
+// (D = 128) clocks of MMA.
 #include <cuda_runtime.h>
 
 #include "attention_tc.cuh"

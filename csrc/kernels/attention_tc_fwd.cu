@@ -1,20 +1,27 @@
 // Masked attention forward on the 5th-generation tensor cores.
 //
 // One CTA holds a tile of 128 rows of queries and walks over its visible keys,
-// KEYS at a time: S = Q K^T into TMEM, softmax with the running maximum and sum in
+// 64 at a time: S = Q K^T into TMEM, softmax with the running maximum and sum in
 // registers, P as 16-bit values back into TMEM over the scores they came from, O += P V
 // with P as the TMEM operand.  S, P and O never leave the SM.
 //
-//   softmax warps   a thread takes 64 scores of a row: one warpgroup for 64 keys, two for 128
-//   last warp       copies through tensor maps and MMAs (and clears padding rows of a tile)
+//   warps 0-3  softmax: a thread takes the 64 scores of a row
+//   warp 4     copies of K and V (and Q, D = 128) through tensor maps
+//   warp 5     MMAs; clears padding rows of a tile
+//
+// S has two places in TMEM: the scores of the tile after next are formed when this
+// tile's P has been read, so the softmax warps find theirs ready.  D = 64 keeps Q in TMEM
+// as well: an instruction with one operand in shared memory takes 44 clocks
+// for 64 keys, with two 74.  Two CTAs share an SM (256 TMEM columns each), one's start
+// and end beside the other's work.
 //
 // What bounds it: a score costs one exponential, 16 a clock and SM, and 4 D
-// operations, 8192 a clock and SM, so up to D = 128 the exponentials are the
-// floor (D = 64: twice the MMA time).  A warp's way through a tile (wait, TMEM load,
-// maximum, exponentials, TMEM store, wait for the product) is mostly latency, so what
-// counts is how many warps an SM has under way: 16, as four CTAs of 128 TMEM columns for
-// D = 64 and two CTAs of 256 columns for D = 128.  With 8 warps an SM (128 scores a
-// thread) the exponential pipe was busy 54 % of the time.
+// operations.  A tile of 64 keys takes a warp 1500 clocks, 700 of them exponentials, the
+// rest latency (TMEM load 80, maximum 100, two votes, TMEM store 60, barriers): two
+// warps a scheduler keep the exponential pipe busy about 60 % of the time.  16 heads x
+// 4096 rows, causal: D = 64 71 us (480 TFLOP/s), with distance bias 90 us; D = 128 91 us
+// (750 TFLOP/s, MMA bound: S with both operands in shared memory), capped 131 us.
+// A CTA costs 6000 to 7000 clocks besides its tiles.
 //
 // The running maximum is only followed when it grows by more than 4 (a factor of
 // 16 in P), so most tiles do not touch O; the sum uses the same reference, so the

@@ -548,3 +548,9 @@ def test_rotary_empty_and_refusals(cuda):
 
 def test_extension_runs_the_operators(cuda):
     assert _ext.available() and hasattr(_ext._C, "attention_forward")
+
+
+def test_no_wait_ran_out(cuda):
+    """Every wait of the tensor-core kernels is bounded; none of this file's calls reached the bound."""
+    torch.cuda.synchronize()
+    assert _ext._C.attention_status() == 0
