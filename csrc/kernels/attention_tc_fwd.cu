@@ -520,6 +520,25 @@ bool packs(const AttnParams& p) { return p.hq > p.hk && p.hq / p.hk * p.sq <= kA
 
 }  // namespace
 
+namespace {
+
+// The driver's encoder, looked up at run time: the module has to load on machines without a driver.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+    return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(p) : nullptr;
+  }();
+  return f;
+}
+
+}  // namespace
+
 bool attn_map(CUtensorMap* m, const AttnTensor& t, const AttnParams& p, int heads, int len, int box_rows, int box_heads) {
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.d), static_cast<cuuint64_t>(len), static_cast<cuuint64_t>(heads),
                               static_cast<cuuint64_t>(p.b)};
@@ -527,7 +546,9 @@ bool attn_map(CUtensorMap* m, const AttnTensor& t, const AttnParams& p, int head
                                  static_cast<cuuint64_t>(t.sb) * 2};
   const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_heads), 1};
   const cuuint32_t ones[4] = {1, 1, 1, 1};
-  return cuTensorMapEncodeTiled(m, p.dt == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+  const EncodeTiled encode = encoder();
+  if (encode == nullptr) return false;
+  return encode(m, p.dt == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                                 t.ptr, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
