@@ -65,6 +65,7 @@ struct AttnParams {
   int splits, split_tiles;
   float* part_o;    // [splits][B][Hq][Sq][D]
   float* part_lse;  // [splits][B][Hq][Sq]
+  int64_t wait_limit;  // clocks that a wait of a tensor-core kernel may last; 0: the wait for scores runs out
   DType dt;
 };
 
@@ -90,6 +91,10 @@ cudaError_t attention_tc_backward(const AttnParams& p, cudaStream_t s);
 // 0, or 1 once a wait of a tensor-core kernel on the current device ran out (its
 // outputs are NaN then); `reset` clears it.  Waits for the device.
 int attention_status(bool reset);
+
+// Limit of later launches' waits, of every device; returns the one before (at first about 4 s).  With 0 the
+// barriers of the scores expect an arrival that never comes, so that their waits run out in every block.
+int64_t attention_wait_limit(int64_t clocks);
 
 }  // namespace launch
 }  // namespace bitscom_b200

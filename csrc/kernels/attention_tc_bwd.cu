@@ -64,9 +64,9 @@ struct Barriers {
   uint64_t full[3], empty[3];
 };
 
-__device__ __forceinline__ void init_barriers(Barriers& bar) {
+__device__ __forceinline__ void init_barriers(Barriers& bar, int64_t wait_limit) {
   mbar_init(&bar.fixed_full, 1);
-  mbar_init(&bar.s_full, 1);
+  mbar_init(&bar.s_full, wait_limit == 0 ? 2 : 1);
   mbar_init(&bar.s_free, kCompute);
   mbar_init(&bar.p_full, kCompute);
   mbar_init(&bar.dp_full, 1);
@@ -79,6 +79,24 @@ __device__ __forceinline__ void init_barriers(Barriers& bar) {
     mbar_init(&bar.empty[i], 1);
   }
   mbar_init_fence();
+}
+
+// Behind the barrier at which the roles meet: whether no wait ran out, in which case all copies and products
+// are over.  Else they are waited for here, for the whole block, before their places are used again.
+// `fixed`: the fixed tiles were copied; `loads`: stages copied.
+template <int STAGES>
+__device__ __forceinline__ bool over(Barriers& bar, const volatile int* raised, bool fixed, int loads, int warp) {
+  if (!*raised) return true;
+  if (warp == kCopier && elect_one()) {
+    if (fixed) Guard::drain(&bar.fixed_full, 0);
+    for (int j = max(0, loads - STAGES); j < loads; ++j) Guard::drain(&bar.full[j % STAGES], (j / STAGES) & 1);
+  }
+  if (warp == kIssuer && elect_one()) {
+    mma_commit(&bar.drain);
+    Guard::drain(&bar.drain, 0);
+  }
+  __syncthreads();
+  return false;
 }
 
 // The products, from descriptors of whole tiles (an instruction takes 16 values of the
@@ -143,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ char smem_raw[];
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int raised;
+  __shared__ int raised, loads;
   __shared__ float partial[4][kAttnTile];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* sq = base;
@@ -173,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(&tmem_slot, 512);
   } else if (warp == kCopier) {  // the first copies are under way before the block meets
     if (elect_one()) {
-      raised = 0;
-      init_barriers(bar);
+      raised = loads = 0;
+      init_barriers(bar, p.wait_limit);
       if (n > 0) {
         mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
         for (int c = 0; c < D / 64; ++c) {
@@ -190,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const Guard guard{&raised, bp.status};
+  const Guard guard{&raised, bp.status, p.wait_limit};
   bool ok = true;
 
   if (warp == kCopier) {
@@ -200,10 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!guard.wait(&bar.empty[j % S::kStages], ((j / S::kStages) & 1) ^ 1)) break;
         load(j);
       }
-      if (raised) {  // no copy may be in flight when the block leaves
-        Guard::drain(&bar.fixed_full, 0);
-        for (int i = max(0, j - S::kStages); i < j; ++i) Guard::drain(&bar.full[i % S::kStages], (i / S::kStages) & 1);
-      }
+      loads = j;
     }
     __syncwarp();
   } else if (warp == kIssuer) {
@@ -261,13 +276,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_rows<16>(tmem + kColDQ, tmem + kColDS, dkv_rows + stage(j), kRows, j > 0);
           mma_commit(&bar.empty[j % S::kStages]);
           mma_commit(&bar.second_done);
-        }
-        __syncwarp();
-      }
-      if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (elect_one()) {
-          mma_commit(&bar.drain);
-          Guard::drain(&bar.drain, 0);
         }
         __syncwarp();
       }
@@ -390,7 +398,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
   }
-  __syncthreads();  // all copies and products are over: Q's place takes the result
+  __syncthreads();
+  ok = over<S::kStages>(bar, &raised, n > 0, loads, warp);  // Q's place takes the result
   if (warp < 8) {
     const int half = warp / 4, row = (warp % 4) * 32 + lane;
     stage_tmem_row<T, D / 2>(tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + kColDQ + half * (D / 2), sq, row,
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ char smem_raw[];
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int raised, first_tile, last_tile;
+  __shared__ int raised, loads, first_tile, last_tile;
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* sk = base;
   char* sv = base + S::kTileBytes;
@@ -473,10 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(&tmem_slot, 512);
   } else if (warp == kCopier) {  // the first copies are under way before the block meets
     if (elect_one()) {
-      raised = 0;
+      raised = loads = 0;
       first_tile = 0x7fffffff;
       last_tile = -1;
-      init_barriers(bar);
+      init_barriers(bar, p.wait_limit);
       mbar_arrive_expect_tx(&bar.fixed_full, 2 * S::kTileBytes);
       for (int c = 0; c < D / 64; ++c) {
         tma_load_4d(sk + c * kAttnTile * 128, &map_k, &bar.fixed_full, c * 64, key0, hk, b);
@@ -506,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   const uint32_t tmem = tmem_slot;
-  const Guard guard{&raised, bp.status};
+  const Guard guard{&raised, bp.status, p.wait_limit};
   bool ok = true;
   RowTiles it{&p, b, key0, first_tile, last_tile, group, 0, 0, false};
   if (p.plan.tile == nullptr) {
@@ -534,11 +543,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.plan.range != nullptr)
           bulk_g2s(rd + 1024, p.plan.range + (static_cast<int64_t>(b) * bp.nq + it.t) * kAttnTile, 1024, &bar.full[st]);
       }
-      if (raised) {  // no copy may be in flight when the block leaves
-        for (int i = max(0, j - S::kStages); i < j; ++i) Guard::drain(&bar.full[i % S::kStages], (i / S::kStages) & 1);
-      }
+      loads = j;
     }
-    if (!some || raised) Guard::drain(&bar.fixed_full, 0);
+    if (!some) Guard::drain(&bar.fixed_full, 0);
     __syncwarp();
   } else if (warp == kIssuer) {
     if (some) {
@@ -624,13 +631,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             products(j + 1);
           }
         }
-      }
-      if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (elect_one()) {
-          mma_commit(&bar.drain);
-          Guard::drain(&bar.drain, 0);
-        }
-        __syncwarp();
       }
     }
   } else {
@@ -749,7 +749,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
   }
-  __syncthreads();  // all copies and products are over: the places of K and V take their gradients
+  __syncthreads();
+  ok = over<S::kStages>(bar, &raised, true, loads, warp);  // the places of K and V take their gradients
   if (warp < 8) {
     const int col = warp / 4 * (D / 2), row = (warp % 4) * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
@@ -803,6 +804,7 @@ namespace launch {
 
 cudaError_t attention_tc_backward(const AttnParams& p, cudaStream_t s) {
   BwdParams bp{p, ScoreScale::of(p), (p.sq + kAttnTile - 1) / kAttnTile, (p.sk + kAttnTile - 1) / kAttnTile, attn_status_ptr()};
+  bp.a.wait_limit = attn_wait_limit();
   if (p.dt == kBF16) return p.d <= 64 ? by_scores<__nv_bfloat16, 64>(bp, s) : by_scores<__nv_bfloat16, 128>(bp, s);
   return p.d <= 64 ? by_scores<__half, 64>(bp, s) : by_scores<__half, 128>(bp, s);
 }

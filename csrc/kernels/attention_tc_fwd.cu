@@ -34,7 +34,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstring>
+#include <atomic>
 
 #include "attention_tc.cuh"
 #include "attention_tc_host.h"
@@ -44,6 +44,7 @@ namespace bitscom_b200 {
 namespace {
 
 __device__ int attn_status = 0;
+std::atomic<int64_t> wait_limit{kWaitLimitClocks};
 
 constexpr float kFollow = 4.f;
 constexpr int kCols = 64;  // scores of a row that a thread takes
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
   extern __shared__ char smem_raw[];
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int raised;
+  __shared__ int raised, loads_k, loads_v;
   char* sq = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* sk = sq + S::kQBytes;
   char* sv = sk + kStages * S::kTileBytes;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
     tmem_alloc(&tmem_slot, S::kTmem);
   } else if (warp == kCopier) {
     if (elect_one()) {
-      raised = 0;
+      raised = loads_k = loads_v = 0;
       for (int c = 0; c < kStages; ++c) {
         mbar_init(&bar.k_full[c], 1);
         mbar_init(&bar.k_empty[c], 1);
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
       mbar_init(&bar.o_full, 1);
       mbar_init(&bar.drain, 1);
       for (int c = 0; c < 2; ++c) {
-        mbar_init(&bar.s_full[c], 1);
+        mbar_init(&bar.s_full[c], p.wait_limit == 0 ? 2 : 1);
         mbar_init(&bar.p_full[c], S::kSoftmax);
       }
       mbar_init_fence();
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const Guard guard{&raised, fp.status};
+  const Guard guard{&raised, fp.status, p.wait_limit};
 
   if (warp == kCopier) {
     if (n > 0 && elect_one()) {
@@ -195,11 +196,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
         load_v(j);
         ++v_loads;
       }
-      if (raised) {  // no copy may be in flight when the block leaves
-        if (!S::kTmemQ) Guard::drain(&bar.q_full, 0);
-        for (int i = max(0, k_loads - kStages); i < k_loads; ++i) Guard::drain(&bar.k_full[i % kStages], (i / kStages) & 1);
-        for (int i = max(0, v_loads - kStages); i < v_loads; ++i) Guard::drain(&bar.v_full[i % kStages], (i / kStages) & 1);
-      }
+      loads_k = k_loads;
+      loads_v = v_loads;
     }
     __syncwarp();
   } else if (warp == kIssuer) {
@@ -270,13 +268,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
           if (!(ok = ok && guard.wait_warp(&bar.pv_done, j & 1))) break;
           scores(j + 2);
         }
-      }
-      if (!ok) {  // no MMA may be in flight when TMEM is freed
-        if (elect_one()) {
-          mma_commit(&bar.drain);
-          Guard::drain(&bar.drain, 0);
-        }
-        __syncwarp();
       }
     }
   } else {
@@ -379,7 +370,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
     const float f = !ok ? __int_as_float(0x7fc00000) : (none ? 0.f : 1.f / l);
     const int64_t row = (static_cast<int64_t>(b) * p.hq + head) * p.sq + i;
     const bool staged = ok && !fp.packed && p.splits == 1;
-    // The copies are done and read by now, their place takes the warp's 32 rows, sub-tiles of 64 columns.
+    // With o_full all copies are done and read, their place takes the warp's 32 rows, sub-tiles of 64 columns.
     char* tile = sk + warp * 4096 * (D / 64);
     char* low = tile + kAttnTile * D * 2;
     if (__any_sync(0xffffffffu, valid)) {
@@ -443,6 +434,18 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (raised) {  // a wait ran out: no copy or MMA may be in flight when TMEM is freed and the block leaves
+    if (warp == kCopier && elect_one()) {
+      if (!S::kTmemQ && n > 0) Guard::drain(&bar.q_full, 0);
+      for (int j = max(0, loads_k - kStages); j < loads_k; ++j) Guard::drain(&bar.k_full[j % kStages], (j / kStages) & 1);
+      for (int j = max(0, loads_v - kStages); j < loads_v; ++j) Guard::drain(&bar.v_full[j % kStages], (j / kStages) & 1);
+    }
+    if (warp == kIssuer && elect_one()) {
+      mma_commit(&bar.drain);
+      Guard::drain(&bar.drain, 0);
+    }
+    __syncthreads();
+  }
   if (warp == kIssuer) tmem_free(tmem, S::kTmem);
 }
 
@@ -554,6 +557,8 @@ bool attn_map(CUtensorMap* m, const AttnTensor& t, const AttnParams& p, int head
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int64_t attn_wait_limit() { return wait_limit.load(); }
+
 int* attn_status_ptr() {
   int* p = nullptr;
   cudaGetSymbolAddress(reinterpret_cast<void**>(&p), attn_status);
@@ -569,6 +574,8 @@ int attention_status(bool reset) {
   if (reset) cudaMemcpyToSymbol(attn_status, &zero, sizeof(int));
   return v;
 }
+
+int64_t attention_wait_limit(int64_t clocks) { return wait_limit.exchange(clocks); }
 
 // Key ranges of a forward launch.  Splitting pays when the row tiles leave most
 // of the two CTA places an SM empty; a split of fewer than four tiles would
@@ -595,6 +602,7 @@ cudaError_t attention_tc_forward(const AttnParams& p, cudaStream_t s) {
   fp.packed = packs(p);
   fp.tiles_q = fp.packed ? 1 : (p.sq + kAttnTile - 1) / kAttnTile;
   fp.status = attn_status_ptr();
+  fp.a.wait_limit = attn_wait_limit();
   if (p.dt == kBF16) return p.d <= 64 ? by_scores<__nv_bfloat16, 64>(fp, s) : by_scores<__nv_bfloat16, 128>(fp, s);
   return p.d <= 64 ? by_scores<__half, 64>(fp, s) : by_scores<__half, 128>(fp, s);
 }

@@ -11,7 +11,10 @@ namespace bitscom_b200 {
 // strides of dimensions longer than one are multiples of 16 bytes (the caller's check).
 bool attn_map(CUtensorMap* m, const AttnTensor& t, const AttnParams& p, int heads, int len, int box_rows, int box_heads);
 
-// The status word of the current device (see attn_status).
+// The status word of the current device (see attention_status).
 int* attn_status_ptr();
+
+// Clocks that a wait of the next launch may last.
+int64_t attn_wait_limit();
 
 }  // namespace bitscom_b200

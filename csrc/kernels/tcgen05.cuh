@@ -29,14 +29,17 @@ namespace bitscom_b200 {
 // ---------------------------------------------------------------------------
 // Bounded waits.  Every wait of a kernel goes through a Guard: a wait that lasts
 // longer than the limit raises a flag in shared memory and a status word, and
-// all other waits of the block then return too; the kernel leaves its loops,
-// waits for its own copies, frees its TMEM and returns.
+// all other waits of the block then return too.  The kernel leaves its loops and
+// the block meets; only then is the flag final, and if it is up the issuers of copies and
+// products wait for all of them before shared memory is used again, TMEM is
+// freed or the block leaves.
 // ---------------------------------------------------------------------------
 constexpr long long kWaitLimitClocks = 8000000000ll;  // about 4 s
 
 struct Guard {
   volatile int* raised;  // shared memory
   int* status;           // global memory
+  long long limit;       // clocks
 
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
     return mbar_try_wait(bar, parity) || wait_long(bar, parity);
@@ -48,7 +51,7 @@ struct Guard {
       for (int i = 0; i < 64; ++i)
         if (mbar_try_wait(bar, parity)) return true;
       if (*raised) return false;
-      if (clock64() - start > kWaitLimitClocks) {
+      if (clock64() - start > limit) {
         *raised = 1;
         atomicExch(status, 1);
         return false;
@@ -59,7 +62,7 @@ struct Guard {
   __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) const {
     return __all_sync(0xffffffffu, wait(bar, parity));
   }
-  // After the flag: for copies in flight, whose barriers complete by themselves.
+  // After the flag: for copies and products in flight, whose barriers complete by themselves.
   __device__ __forceinline__ static void drain(uint64_t* bar, uint32_t parity) {
     const long long start = clock64();
     while (!mbar_try_wait(bar, parity))

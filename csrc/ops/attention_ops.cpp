@@ -483,6 +483,9 @@ void register_attention_bindings(pybind11::module_& m) {
         py::arg("causal"), py::arg("scale"), py::arg("cap"));
   m.def("attention_status", [](bool reset) { return launch::attention_status(reset); }, py::arg("reset") = false,
         "1 once a wait of a tensor-core attention kernel on the current device ran out, else 0 (waits for the device).");
+  m.def("attention_wait_limit", &launch::attention_wait_limit, py::arg("clocks"),
+        "Sets how many clocks a wait inside a tensor-core attention kernel may last before the kernel gives up (0: the "
+        "wait for scores always runs out, for tests of that path); returns the limit before.");
   m.def("rotary_forward", &rotary_forward, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
         py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
   m.def("rotary_train", &rotary_train, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
