@@ -177,6 +177,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       q[c] = valid && c * 8 < p.d ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+  } else if (!S::kTmemQ && fp.packed && !valid) {
+    // The copy of packed rows leaves the tile's other rows as the last kernel left them; their scores take
+    // part in the warp's votes (which tanh, whether the maximum is followed), so they are zeros.
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        *reinterpret_cast<uint4*>(sq + c * kAttnTile * 128 + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
