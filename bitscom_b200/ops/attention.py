@@ -124,9 +124,9 @@ def attention(
         documents, prefix: see the module's description and
             :func:`attention_mask`, which builds them into a ``mask`` once for
             several calls; ``mask`` replaces ``causal``, ``documents``, ``prefix``.
-        softcap: cap of the scores (> 0), None for none.
+        softcap: cap of the scores (1e-30 to 1e30), None for none.
         slopes: ``[heads]`` distance slopes (not differentiated).
-        scale: factor of ``q.k`` (> 0), default ``head size ** -0.5``.
+        scale: factor of ``q.k`` (1e-30 to 1e30), default ``head size ** -0.5``.
 
     Returns ``[batch, heads, q_len, head size]`` in q's dtype (stored
     ``[batch, q_len, heads, head size]``).  Rows that see no key are zero, with
@@ -137,10 +137,10 @@ def attention(
     type for the products; all sums are float32.  Under autocast float32 inputs
     are cast like those of torch's own attention.
     """
-    if softcap is not None and not softcap > 0:
-        raise ValueError(f"softcap must be positive, got {softcap}")
-    if scale is not None and not scale > 0:
-        raise ValueError(f"scale must be positive, got {scale}")
+    if softcap is not None and not 1e-30 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be positive, from 1e-30 to 1e30, got {softcap}")
+    if scale is not None and not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale must be positive, from 1e-30 to 1e30, got {scale}")
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention does not differentiate slopes: detach them")
     if torch.is_autocast_enabled(q.device.type):

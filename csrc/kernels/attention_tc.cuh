@@ -1,6 +1,8 @@
 // Shared parts of the tensor-core attention kernels (forward and backward).
 #pragma once
 
+#include <algorithm>
+
 #include "attention_common.cuh"
 #include "tcgen05.cuh"
 
@@ -27,22 +29,27 @@ struct ScoreScale {
   float cap_in;   // capped: 2 log2 e * scale / cap
   float cap_out;  // capped: cap * log2 e
   float cap_inv;  // capped: 1 / cap_out
-  float near, mid;          // capped: largest raw scores of the polynomials
+  float near, mid;          // capped: largest raw scores of the polynomials, -1: not used
   float poly3[3], poly5[5];  // capped: the polynomials for raw scores, times cap_out
+  // In double, as powers of scale / cap leave the range of fp32 for caps that are accepted.
   static ScoreScale of(const AttnParams& p) {
+    constexpr double most = 3.4028234663852886e38;  // of fp32
+    constexpr double square = 1e18;                 // what the polynomials can square
     ScoreScale s{};
     s.c = p.scale * kLog2e;
     if (p.cap > 0.f) {
-      const float k = p.scale / p.cap;
-      s.cap_out = p.cap * kLog2e;
-      s.cap_in = 2.f * kLog2e * k;
-      s.cap_inv = 1.f / s.cap_out;
-      s.near = kTanhNear / k;
-      s.mid = kTanhMid / k;
-      float f = k * s.cap_out;
+      const double k = static_cast<double>(p.scale) / p.cap, out = static_cast<double>(p.cap) * kLog2e;
+      s.cap_out = static_cast<float>(out);
+      s.cap_in = static_cast<float>(std::min(2. * kLog2e * k, most));
+      s.cap_inv = static_cast<float>(1. / out);
+      s.near = static_cast<float>(std::min(kTanhNear / k, square));
+      s.mid = static_cast<float>(std::min(kTanhMid / k, square));
+      double f = k * out;
       for (int i = 0; i < 5; ++i, f *= k * k) {
-        if (i < 3) s.poly3[i] = kTanhPoly3[i] * f;
-        s.poly5[i] = kTanhPoly5[i] * f;
+        if (i < 3) s.poly3[i] = static_cast<float>(std::min(std::max(kTanhPoly3[i] * f, -most), most));
+        s.poly5[i] = static_cast<float>(std::min(std::max(kTanhPoly5[i] * f, -most), most));
+        if (f > 1e38 && i < 3) s.near = -1.f;
+        if (f > 1e38) s.mid = -1.f;
       }
     }
     return s;
@@ -99,9 +106,6 @@ __device__ __forceinline__ void bias_scores(float (&s)[N], float factor, float s
     for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, -slope * fabsf(d0 + c));
   }
 }
-
-// A score that counts as nothing, finite so that products with its zero weight are zero.
-constexpr float kMasked = -1e15f;
 
 // Clears the rows of an operand tile that `dead` names: sub-tiles of 64 columns and ROWS rows.
 template <int ROWS>

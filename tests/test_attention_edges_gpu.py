@@ -8,6 +8,8 @@ import torch
 import bitscom_b200 as bitscom
 from bitscom_b200 import _ext
 
+from .attention_oracle import check, reference, visible
+
 pytestmark = pytest.mark.gpu
 
 
@@ -71,3 +73,28 @@ def test_shared_memory_of_another_call_does_not_show(cuda, dtype):
         bitscom.attention(other[0] * scale, other[1], other[2], causal=False, softcap=30.0)
         outs.append(bitscom.attention(q * 0.5, k, v, softcap=30.0))
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e-5, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64)], ids=str)
+def test_caps_far_below_the_scores(cuda, dtype, d, cap):
+    """Scores of +-cap: nearly even weights, and no gradient through the scores but where one is near zero."""
+    for causal, ids in ((True, None), (True, torch.arange(200).div(70, rounding_mode="floor").repeat(2, 1))):
+        q, k, v, do = _qkv(2, 4, 2, 200, 200, d, dtype, grad=True)
+        out = bitscom.attention(q, k, v, causal=causal, documents=None if ids is None else ids.cuda(), softcap=cap)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        vals, bounds = reference(q, k, v, do, seen=visible(2, 200, 200, causal, ids), softcap=cap)
+        # The gradient's factor 1 - tanh^2 of a score x is a step at x = 0, as wide as the cap: where the fp32 score's
+        # rounding (below 2 d sum|q||k| 2^-24) can cross it, all of ds is open.
+        check({"out": out, "dv": grads[2]}, vals, bounds)
+        assert all(torch.isfinite(x).all() for x in grads[:2])
+
+
+def test_caps_far_above_the_scores(cuda):
+    """A cap that no score comes near changes nothing beyond rounding, up to the largest accepted."""
+    q, k, v, do = _qkv(1, 4, 2, 200, 200, 64, torch.float16, grad=True)
+    vals, bounds = reference(q, k, v, do, seen=visible(1, 200, 200, True))
+    for cap in (1e6, 1e12, 1e25, 1e30):
+        out = bitscom.attention(q, k, v, softcap=cap)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        check(dict(zip(("out", "dq", "dk", "dv"), (out, *grads))), vals, bounds)
