@@ -133,6 +133,7 @@ def attention(
     zero gradients.  Keys that no query may see because they are padding are
     never touched by the arithmetic, whatever they hold; a NaN or infinity in
     any other key can reach every query whose tile of 128 keys holds it.
+    Gradients are by the backward pass, once; on CUDA a forward-mode tangent is refused.
     float16 and bfloat16 round the probabilities and score gradients to that
     type for the products; all sums are float32.  Under autocast float32 inputs
     are cast like those of torch's own attention.

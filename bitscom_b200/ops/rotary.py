@@ -53,7 +53,8 @@ def qk_norm_rotary(
             (i, i + rotated / 2).
 
     Arithmetic is float32 with one rounding at the end.  Gradients reach q, k
-    and the gains (summed in a fixed order), not frequencies or positions.
+    and the gains (summed in a fixed order), not frequencies or positions; on CUDA
+    a forward-mode tangent is refused.
     """
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise ValueError("qk_norm_rotary does not differentiate frequencies: detach them")

@@ -39,6 +39,13 @@ int int_bytes(const at::Tensor& t, const char* name) {
   return t.scalar_type() == at::kLong ? 8 : 4;
 }
 
+// The operators have no forward-mode derivative: a tangent is refused, not dropped.
+void no_tangents(std::initializer_list<OptTensor> tensors) {
+  for (const auto& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has(t) || !t->_fw_grad(0).defined(),
+                                "bitscom: the attention operators have no forward-mode derivative");
+}
+
 cudaStream_t stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // ---------------------------------------------------------------------------
@@ -167,6 +174,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tenso
             const at::Tensor& v_in, const OptTensor& plan,
                                                                  const OptTensor& slopes, bool causal, double scale,
                                                                  double cap, bool want_lse) {
+  no_tangents({q_in, k_in, v_in, slopes});
   check_qkv(q_in, k_in, v_in);
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
@@ -322,6 +330,7 @@ RotaryCall rotary_call(const at::Tensor& q, const at::Tensor& k, const at::Tenso
 std::tuple<at::Tensor, at::Tensor> rotary_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
                                                   const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
                                                   double eps, bool interleaved) {
+  no_tangents({q, k, freq, wq, wk});
   RotaryCall c = rotary_call(q, k, freq, wq, wk, positions, eps, interleaved);
   c10::cuda::CUDAGuard g(q.device());
   auto oq = at::empty(q.sizes(), q.options()), ok = at::empty(k.sizes(), k.options());

@@ -4,6 +4,7 @@ Needs a CUDA device."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import bitscom_b200 as bitscom
 from bitscom_b200 import _ext
@@ -98,3 +99,34 @@ def test_caps_far_above_the_scores(cuda):
         out = bitscom.attention(q, k, v, softcap=cap)
         grads = torch.autograd.grad(out, (q, k, v), do)
         check(dict(zip(("out", "dq", "dk", "dv"), (out, *grads))), vals, bounds)
+
+
+def test_forward_mode_is_refused(cuda):
+    """The operators have no forward-mode derivative: a dual input is refused, never taken as a constant."""
+    q, k, v, t = _qkv(1, 2, 2, 20, 20, 64, torch.float16)
+    freq = bitscom.rotary_frequencies(64, device="cuda")
+    gain = torch.ones(64, device="cuda")
+    slopes = torch.ones(2, device="cuda")
+    with fwad.dual_level():
+        dual = fwad.make_dual(q, t)
+        bad = [
+            lambda: bitscom.attention(dual, k, v),
+            lambda: bitscom.attention(q, fwad.make_dual(k, t), v),
+            lambda: bitscom.attention(q, k, fwad.make_dual(v, t), softcap=3.0),
+            lambda: bitscom.attention(q, k, v, slopes=fwad.make_dual(slopes, slopes)),
+            lambda: bitscom.attention(dual, k.detach().requires_grad_(True), v),
+            lambda: bitscom.qk_norm_rotary(dual, k, freq),
+            lambda: bitscom.qk_norm_rotary(q, fwad.make_dual(k, t), freq),
+            lambda: bitscom.qk_norm_rotary(q, k, fwad.make_dual(freq, freq)),
+            lambda: bitscom.qk_norm_rotary(q, k, freq, q_weight=fwad.make_dual(gain, gain)),
+            lambda: bitscom.qk_norm_rotary(q, k, freq, k_weight=fwad.make_dual(gain, gain)),
+        ]
+        for call in bad:
+            with torch.no_grad():
+                with pytest.raises((NotImplementedError, ValueError)):
+                    call()
+            with pytest.raises((NotImplementedError, ValueError)):
+                call()
+        assert fwad.unpack_dual(bitscom.attention(q, k, v)).tangent is None
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda x: bitscom.attention(x, k, v), (q,), (t,))
