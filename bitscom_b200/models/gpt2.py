@@ -57,12 +57,14 @@ class _Attention(nn.Module):
 
     def _constant(self, name: str, device: torch.device) -> torch.Tensor:
         if (name, device) not in self._constants:
-            if name == "frequencies":
-                d = self.qkv.in_features // self.n_head
-                value = rotary_frequencies(d - d % 2)
-            else:
-                value = 2.0 ** (-8.0 * torch.arange(1, self.n_head + 1, dtype=torch.float32) / self.n_head)
-            self._constants[name, device] = value.to(device)
+            # Kept for later calls, training among them, which an inference tensor could not serve.
+            with torch.inference_mode(False):
+                if name == "frequencies":
+                    d = self.qkv.in_features // self.n_head
+                    value = rotary_frequencies(d - d % 2)
+                else:
+                    value = 2.0 ** (-8.0 * torch.arange(1, self.n_head + 1, dtype=torch.float32) / self.n_head)
+                self._constants[name, device] = value.to(device)
         return self._constants[name, device]
 
     def forward(self, x, mask=None):

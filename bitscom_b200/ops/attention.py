@@ -92,11 +92,12 @@ def attention_mask(
     for name, t in (("documents", documents), ("prefix", prefix)):
         if t is not None and t.dtype not in _INTS:
             raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-    if _ext.use_cuda_kernels(like):
-        plan = _ext._C.attention_plan(documents, prefix, causal, batch, q_len, k_len)
-        return AttentionMask(causal, batch, q_len, k_len, plan, None, None)
-    return AttentionMask(causal, batch, q_len, k_len, None, None if documents is None else documents.clone(),
-                         None if prefix is None else prefix.clone())
+    with torch.inference_mode(False):  # a mask made in inference mode serves training too
+        if _ext.use_cuda_kernels(like):
+            plan = _ext._C.attention_plan(documents, prefix, causal, batch, q_len, k_len)
+            return AttentionMask(causal, batch, q_len, k_len, plan, None, None)
+        return AttentionMask(causal, batch, q_len, k_len, None, None if documents is None else documents.clone(),
+                             None if prefix is None else prefix.clone())
 
 
 def attention(

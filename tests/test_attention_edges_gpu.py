@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as fwad
 
 import bitscom_b200 as bitscom
 from bitscom_b200 import _ext
+from bitscom_b200.models import gpt2_small_test
 
 from .attention_oracle import check, reference, visible
 
@@ -130,3 +131,21 @@ def test_forward_mode_is_refused(cuda):
         assert fwad.unpack_dual(bitscom.attention(q, k, v)).tangent is None
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.jvp(lambda x: bitscom.attention(x, k, v), (q,), (t,))
+
+
+@pytest.mark.parametrize("options", [dict(rotary=True), dict(distance_bias=True)], ids=str)
+def test_training_after_inference_mode(cuda, options):
+    """A first forward pass in inference mode leaves nothing behind that a training step cannot use."""
+    torch.manual_seed(0)
+    model = gpt2_small_test(vocab_size=64, n_positions=40, **options).cuda()
+    idx = torch.randint(0, 64, (1, 30), device="cuda")
+    ids = torch.zeros(1, 30, dtype=torch.int32, device="cuda")
+    with torch.inference_mode():
+        want = model(idx, documents=ids)
+        mask = bitscom.attention_mask(ids.clone())
+    out = model(idx, documents=ids)
+    assert torch.equal(out, want)
+    out.square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+    q, k, v, do = _qkv(1, 2, 2, 30, 30, 64, torch.float16, grad=True)
+    torch.autograd.grad(bitscom.attention(q, k, v, mask=mask), (q, k, v), do)
