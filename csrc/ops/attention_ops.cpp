@@ -101,6 +101,10 @@ void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
   TORCH_CHECK_VALUE(q.size(2) < (1 << 30) && k.size(2) < (1 << 30), "bitscom: lengths must be below 2^30");
 }
 
+// As the kernels read them, which is one after another.
+OptTensor slopes_of(const OptTensor& t) { return has(t) ? OptTensor(t->contiguous()) : OptTensor(); }
+
+// The tensors have to outlive the launch: `slopes` is from slopes_of().
 AttnParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
                      const OptTensor& slopes, bool causal, double scale, double cap) {
   AttnParams p{};
@@ -121,9 +125,8 @@ AttnParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   if (has(slopes)) {
     same_device(*slopes, q, "slopes");
     TORCH_CHECK_TYPE(slopes->scalar_type() == at::kFloat, "bitscom: slopes must be float32");
-    TORCH_CHECK_VALUE(slopes->dim() == 1 && slopes->size(0) == q.size(1) && slopes->is_contiguous(),
-                      "bitscom: slopes must be a contiguous vector of one value for each of the ", q.size(1),
-                      " query heads");
+    TORCH_CHECK_VALUE(slopes->dim() == 1 && slopes->size(0) == q.size(1),
+                      "bitscom: slopes must be a vector of one value for each of the ", q.size(1), " query heads");
     p.slopes = slopes->data_ptr<float>();
   }
   if (has(plan)) {
@@ -172,12 +175,13 @@ at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, b
 // Returns (out, log-sums, out's rounding); the last two only when the backward pass wants them.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tensor& q_in, const at::Tensor& k_in,
             const at::Tensor& v_in, const OptTensor& plan,
-                                                                 const OptTensor& slopes, bool causal, double scale,
+                                                                 const OptTensor& slopes_in, bool causal, double scale,
                                                                  double cap, bool want_lse) {
-  no_tangents({q_in, k_in, v_in, slopes});
+  no_tangents({q_in, k_in, v_in, slopes_in});
   check_qkv(q_in, k_in, v_in);
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
+  const OptTensor slopes = slopes_of(slopes_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   auto out = tokens_first(q);
   at::Tensor lse, lo;
@@ -214,7 +218,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tenso
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     const at::Tensor& dout_in, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-    const at::Tensor& out, const at::Tensor& lse, const OptTensor& lo, const OptTensor& plan, const OptTensor& slopes, bool causal,
+    const at::Tensor& out, const at::Tensor& lse, const OptTensor& lo, const OptTensor& plan, const OptTensor& slopes_in, bool causal,
     double scale, double cap) {
   check_qkv(q_in, k_in, v_in);
   same_device(dout_in, q_in, "the output's gradient");
@@ -230,6 +234,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     dv.zero_();
     return {dq, dk, dv};
   }
+  const OptTensor slopes = slopes_of(slopes_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   p.o = view_of(out);
   if (has(lo)) p.lo = view_of(*lo);

@@ -149,3 +149,18 @@ def test_training_after_inference_mode(cuda, options):
     assert all(torch.isfinite(p.grad).all() for p in model.parameters())
     q, k, v, do = _qkv(1, 2, 2, 30, 30, 64, torch.float16, grad=True)
     torch.autograd.grad(bitscom.attention(q, k, v, mask=mask), (q, k, v), do)
+
+
+def test_slopes_of_any_stride(cuda):
+    q, k, v, do = _qkv(1, 4, 2, 130, 130, 64, torch.float16, grad=True)
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    wide = torch.full((4, 3), 9.0, device="cuda")
+    wide[:, 1] = slopes
+    want = bitscom.attention(q, k, v, slopes=slopes)
+    grads = torch.autograd.grad(want, (q, k, v), do)
+    for given in (wide[:, 1], slopes.flip(0).contiguous().flip(0)):
+        got = bitscom.attention(q, k, v, slopes=given)
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (q, k, v), do), grads))
+    same = bitscom.attention(q, k, v, slopes=slopes[:1].expand(4))
+    assert torch.equal(same, bitscom.attention(q, k, v, slopes=torch.full((4,), 0.5, device="cuda")))
