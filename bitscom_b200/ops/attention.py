@@ -139,6 +139,8 @@ def attention(
     type for the products; all sums are float32.  Under autocast float32 inputs
     are cast like those of torch's own attention.
     """
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k and v must be [batch, heads, length, head size]")
     if softcap is not None and not 1e-30 <= softcap <= 1e30:
         raise ValueError(f"softcap must be positive, from 1e-30 to 1e30, got {softcap}")
     if scale is not None and not 1e-30 <= scale <= 1e30:
@@ -189,8 +191,6 @@ def _visible(causal, batch, q_len, k_len, documents, prefix) -> torch.Tensor:
 
 
 def _attention_cpu(q, k, v, mask, causal, slopes, scale, cap):
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError("q, k and v must be [batch, heads, length, head size]")
     if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k and v must have one dtype of {_FLOATS}, got {q.dtype}, {k.dtype} and {v.dtype}")
     if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:

@@ -30,3 +30,11 @@ def test_inference_mode_leaves_no_inference_tensors(options):
     kept = list(model.blocks[0].attn._constants.values()) + [mask.documents, mask.prefix]
     assert len(kept) == 3 and not any(t.is_inference() for t in kept)
     model(idx, documents=ids).sum().backward()
+
+
+def test_wrong_ranks_are_refused_with_masks():
+    q, k, ids = torch.randn(2, 4, 6, 8), torch.randn(2, 2, 6, 8), torch.zeros(2, 6, dtype=torch.int32)
+    for kw in ({}, {"documents": ids}, {"mask": bitscom.attention_mask(ids)}, {"prefix": ids[:, 0]}):
+        for args in ((q[0], k, k), (q[0, 0], k, k), (q, k[0, 0], k), (q, k, k[0, 0])):
+            with pytest.raises(ValueError, match="batch, heads, length"):
+                bitscom.attention(*args, **kw)
