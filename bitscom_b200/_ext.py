@@ -43,3 +43,10 @@ def use_cuda_kernels(t: torch.Tensor) -> bool:
         return False
     require("CUDA tensors")
     return True
+
+
+def operator(name: str):
+    """The operator ``bitscom_b200::name``: its binding, or the form that traces record."""
+    if torch.jit.is_tracing() or torch.compiler.is_compiling():
+        return getattr(torch.ops.bitscom_b200, name)
+    return getattr(_C, name)

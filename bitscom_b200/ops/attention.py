@@ -92,10 +92,10 @@ def attention_mask(
     for name, t in (("documents", documents), ("prefix", prefix)):
         if t is not None and t.dtype not in _INTS:
             raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    if _ext.use_cuda_kernels(like):
+        plan = _ext.operator("attention_plan")(documents, prefix, causal, batch, q_len, k_len)
+        return AttentionMask(causal, batch, q_len, k_len, plan, None, None)
     with torch.inference_mode(False):  # a mask made in inference mode serves training too
-        if _ext.use_cuda_kernels(like):
-            plan = _ext._C.attention_plan(documents, prefix, causal, batch, q_len, k_len)
-            return AttentionMask(causal, batch, q_len, k_len, plan, None, None)
         return AttentionMask(causal, batch, q_len, k_len, None, None if documents is None else documents.clone(),
                              None if prefix is None else prefix.clone())
 
@@ -165,9 +165,7 @@ def attention(
     if mask is not None and mask.plan is None:
         raise ValueError("the mask was built from CPU tensors, q is on " + str(q.device))
     plan = None if mask is None else mask.plan
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _ext._C.attention_train(q, k, v, plan, slopes, causal, scale, cap)
-    return _ext._C.attention_forward(q, k, v, plan, slopes, causal, scale, cap, False)[0]
+    return _ext.operator("attention_forward")(q, k, v, plan, slopes, causal, scale, cap)
 
 
 def _visible(causal, batch, q_len, k_len, documents, prefix) -> torch.Tensor:
@@ -228,6 +226,32 @@ def _attention_cpu(q, k, v, mask, causal, slopes, scale, cap):
     p = torch.softmax(s, -1).masked_fill(none, 0.0) if sk else s
     out = (p @ vf).reshape(b, h, sq, d)
     return out.transpose(1, 2).to(q.dtype).contiguous().transpose(1, 2)
+
+
+if _ext.available():  # what tracing with fake tensors sees: the layouts of csrc/ops/attention_ops.cpp
+
+    def _tokens_first(t):
+        return t.new_empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3])).transpose(1, 2)
+
+    @torch.library.register_fake("bitscom_b200::attention_plan")
+    def _(documents, prefix, causal, batch, q_len, k_len):
+        like = documents if documents is not None else prefix
+        q_tiles, k_tiles = (q_len + 127) // 128, (k_len + 127) // 128
+        return like.new_empty(batch * (q_tiles * (2 * 128 + 8) + k_tiles * 4), dtype=torch.int32)
+
+    @torch.library.register_fake("bitscom_b200::attention_forward")
+    def _(q, k, v, plan, slopes, causal, scale, cap):
+        return _tokens_first(q)
+
+    @torch.library.register_fake("bitscom_b200::attention_forward_sums")
+    def _(q, k, v, plan, slopes, causal, scale, cap):
+        tensor_cores = q.dtype != torch.float32 and q.shape[3] % 8 == 0 and q.shape[3] <= 128
+        sums = q.new_empty(q.shape[:3], dtype=torch.float32)
+        return _tokens_first(q), sums, _tokens_first(q) if tensor_cores else q.new_empty(0)
+
+    @torch.library.register_fake("bitscom_b200::attention_backward")
+    def _(grad, q, k, v, out, sums, low, plan, slopes, causal, scale, cap):
+        return _tokens_first(q), _tokens_first(k), _tokens_first(v)
 
 
 __all__ = ["AttentionMask", "attention", "attention_mask"]

@@ -60,9 +60,7 @@ def qk_norm_rotary(
         raise ValueError("qk_norm_rotary does not differentiate frequencies: detach them")
     if not _ext.use_cuda_kernels(q):
         return _qk_norm_rotary_cpu(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _ext._C.rotary_train(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
-    return _ext._C.rotary_forward(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
+    return _ext.operator("rotary_forward")(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved)
 
 
 def _qk_norm_rotary_cpu(q, k, freq, wq, wk, positions, eps, interleaved):
@@ -108,6 +106,18 @@ def _qk_norm_rotary_cpu(q, k, freq, wq, wk, positions, eps, interleaved):
         return torch.cat((z, y[..., r:]), -1).to(x.dtype)
 
     return one(q, wq), one(k, wk)
+
+
+if _ext.available():  # what tracing with fake tensors sees
+
+    @torch.library.register_fake("bitscom_b200::rotary_forward")
+    def _(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved):
+        return q.new_empty(q.shape), k.new_empty(k.shape)
+
+    @torch.library.register_fake("bitscom_b200::rotary_backward")
+    def _(grad_q, grad_k, q, k, frequencies, q_weight, k_weight, positions, eps, interleaved, want_gains):
+        gains = q.new_empty((2, q.shape[3]) if want_gains else (0,), dtype=torch.float32)
+        return q.new_empty(q.shape), k.new_empty(k.shape), gains
 
 
 __all__ = ["qk_norm_rotary", "rotary_frequencies"]

@@ -1,13 +1,19 @@
-// Argument checks and Python bindings of the attention operators: masked
-// attention (forward, backward, mask plans) and the per-head norm with
+// Argument checks, torch operators and Python bindings of the attention operators:
+// masked attention (forward, backward, mask plans) and the per-head norm with
 // rotation.  Every launch is on the caller's current stream of the tensors'
 // device; workspaces come from the caching allocator on that stream.
+//
+// They are operators of torch's dispatcher (namespace bitscom_b200), so that traces, fake tensors
+// and function transforms see them; the bindings call them through it, which costs
+// less than a call through torch.ops.
 #include "ops/attention_ops.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+#include <torch/library.h>
 
 #include "kernels/attention.h"
 #include "kernels/qk_norm_rotary.h"
@@ -161,6 +167,7 @@ at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, b
   }
   c10::cuda::CUDAGuard g(like.device());
   const at::Tensor pre = has(prefix) ? prefix->contiguous() : at::Tensor();
+  c10::InferenceMode normal(false);  // a plan made in inference mode serves training too
   auto plan = at::empty({PlanView::words(batch, q_len, k_len)}, like.options().dtype(at::kInt));
   if (plan.numel() == 0) return plan;
   launch::attention_plan(has(documents) ? documents->data_ptr() : nullptr, ids_bytes,
@@ -172,12 +179,12 @@ at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, b
   return plan;
 }
 
-// Returns (out, log-sums, out's rounding); the last two only when the backward pass wants them.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tensor& q_in, const at::Tensor& k_in,
-            const at::Tensor& v_in, const OptTensor& plan,
-                                                                 const OptTensor& slopes_in, bool causal, double scale,
-                                                                 double cap, bool want_lse) {
-  no_tangents({q_in, k_in, v_in, slopes_in});
+// Returns (out, log-sums, out's rounding); the last two only for the backward pass, the last one empty where
+// it is not kept.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> run_forward(const at::Tensor& q_in, const at::Tensor& k_in,
+                                                           const at::Tensor& v_in, const OptTensor& plan,
+                                                           const OptTensor& slopes_in, bool causal, double scale,
+                                                           double cap, bool want_sums) {
   check_qkv(q_in, k_in, v_in);
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
@@ -186,20 +193,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tenso
   auto out = tokens_first(q);
   at::Tensor lse, lo;
   const auto f32 = q.options().dtype(at::kFloat);
-  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, f32);
+  if (want_sums) {
+    lse = at::empty({q.size(0), q.size(1), q.size(2)}, f32);
+    lo = for_tensor_cores(q) ? tokens_first(q) : at::empty({0}, q.options());
+  }
   if (out.numel() == 0) return {out, lse, lo};
   if (p.sk == 0) {
     out.zero_();
-    if (want_lse) lse.fill_(std::numeric_limits<float>::infinity());
+    if (want_sums) lse.fill_(std::numeric_limits<float>::infinity());
     return {out, lse, lo};
   }
   p.o = view_of(out);
-  p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  p.lse = want_sums ? lse.data_ptr<float>() : nullptr;
   if (for_tensor_cores(q)) {
-    if (want_lse) {
-      lo = tokens_first(q);
-      p.lo = view_of(lo);
-    }
+    if (want_sums) p.lo = view_of(lo);
     launch::attention_tc_splits(p, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.splits, &p.split_tiles);
     at::Tensor part_o, part_lse;
     if (p.splits > 1) {
@@ -216,10 +223,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tenso
   return {out, lse, lo};
 }
 
+at::Tensor attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
+                             const OptTensor& slopes, bool causal, double scale, double cap) {
+  return std::get<0>(run_forward(q, k, v, plan, slopes, causal, scale, cap, false));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward_sums(const at::Tensor& q, const at::Tensor& k,
+                                                                      const at::Tensor& v, const OptTensor& plan,
+                                                                      const OptTensor& slopes, bool causal,
+                                                                      double scale, double cap) {
+  return run_forward(q, k, v, plan, slopes, causal, scale, cap, true);
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     const at::Tensor& dout_in, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-    const at::Tensor& out, const at::Tensor& lse, const OptTensor& lo, const OptTensor& plan, const OptTensor& slopes_in, bool causal,
-    double scale, double cap) {
+    const at::Tensor& out, const at::Tensor& lse, const at::Tensor& lo, const OptTensor& plan,
+    const OptTensor& slopes_in, bool causal, double scale, double cap) {
   check_qkv(q_in, k_in, v_in);
   same_device(dout_in, q_in, "the output's gradient");
   c10::cuda::CUDAGuard g(q_in.device());
@@ -237,14 +256,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
   const OptTensor slopes = slopes_of(slopes_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   p.o = view_of(out);
-  if (has(lo)) p.lo = view_of(*lo);
   p.dout = view_of(dout);
   p.dq = view_of(dq);
   p.dk = view_of(dk);
   p.dv = view_of(dv);
   p.lse = lse.data_ptr<float>();
   if (for_tensor_cores(q)) {
-    TORCH_CHECK(has(lo), "bitscom: the forward pass kept no rounding of its output");
+    TORCH_CHECK(lo.sizes() == out.sizes(), "bitscom: the forward pass kept no rounding of its output");
+    p.lo = view_of(lo);
     const int64_t tiles = (q.size(2) + kAttnTile - 1) / kAttnTile;
     auto stats = at::empty({q.size(0), q.size(1), tiles, 2, kAttnTile}, lse.options());
     p.stats = stats.data_ptr<float>();
@@ -335,7 +354,6 @@ RotaryCall rotary_call(const at::Tensor& q, const at::Tensor& k, const at::Tenso
 std::tuple<at::Tensor, at::Tensor> rotary_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
                                                   const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
                                                   double eps, bool interleaved) {
-  no_tangents({q, k, freq, wq, wk});
   RotaryCall c = rotary_call(q, k, freq, wq, wk, positions, eps, interleaved);
   c10::cuda::CUDAGuard g(q.device());
   auto oq = at::empty(q.sizes(), q.options()), ok = at::empty(k.sizes(), k.options());
@@ -346,7 +364,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_forward(const at::Tensor& q, const at:
   return {oq, ok};
 }
 
-// Returns (dq, dk, dw [2, D] fp32 or undefined).
+// Returns (dq, dk, dw [2, D] fp32, empty when not wanted).
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rotary_backward(const at::Tensor& gq_in, const at::Tensor& gk_in,
                                                                const at::Tensor& q, const at::Tensor& k,
                                                                const at::Tensor& freq, const OptTensor& wq,
@@ -369,8 +387,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rotary_backward(const at::Tensor&
   c.p.ok = heads_of(dk);
   c.p.gq = heads_of(gq);
   c.p.gk = heads_of(gk);
-  at::Tensor dw, partial;
+  at::Tensor partial;
   const auto f32 = q.options().dtype(at::kFloat);
+  at::Tensor dw = at::empty({0}, f32);
   if (want_dw) {
     if (c.p.tokens == 0) {
       dw = at::zeros({2, q.size(3)}, f32);
@@ -384,6 +403,28 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rotary_backward(const at::Tensor&
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dw};
 }
+
+// ---------------------------------------------------------------------------
+// The operators below autograd, as the nodes and bindings call them.
+// ---------------------------------------------------------------------------
+template <auto Impl, const char* Name>
+struct Op;
+template <typename R, typename... A, R (*Impl)(A...), const char* Name>
+struct Op<Impl, Name> {
+  static R call(A... a) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(Name, "").template typed<R(A...)>();
+    return op.call(std::forward<A>(a)...);
+  }
+};
+constexpr char kPlan[] = "bitscom_b200::attention_plan", kForward[] = "bitscom_b200::attention_forward",
+               kForwardSums[] = "bitscom_b200::attention_forward_sums", kBackward[] = "bitscom_b200::attention_backward",
+               kRotary[] = "bitscom_b200::rotary_forward", kRotaryBackward[] = "bitscom_b200::rotary_backward";
+using PlanOp = Op<&attention_plan, kPlan>;
+using ForwardOp = Op<&attention_forward, kForward>;
+using ForwardSumsOp = Op<&attention_forward_sums, kForwardSums>;
+using BackwardOp = Op<&attention_backward, kBackward>;
+using RotaryOp = Op<&rotary_forward, kRotary>;
+using RotaryBackwardOp = Op<&rotary_backward, kRotaryBackward>;
 
 // ---------------------------------------------------------------------------
 // Autograd nodes, in C++: a training call of small tensors is bound by the host.
@@ -419,7 +460,8 @@ variable_list once(variable_list grads, const variable_list& sources) {
 struct Attention : public torch::autograd::Function<Attention> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const OptTensor& plan, const OptTensor& slopes, bool causal, double scale, double cap) {
-    auto [out, lse, lo] = attention_forward(q, k, v, plan, slopes, causal, scale, cap, true);
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, lse, lo] = ForwardSumsOp::call(q, k, v, plan, slopes, causal, scale, cap);
     ctx->save_for_backward({q, k, v, out, lse, lo, or_undefined(plan), or_undefined(slopes)});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
@@ -431,9 +473,9 @@ struct Attention : public torch::autograd::Function<Attention> {
     variable_list d;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dq, dk, dv] = attention_backward(g[0], s[0], s[1], s[2], s[3], s[4], if_defined(s[5]), if_defined(s[6]),
-                                             if_defined(s[7]), ctx->saved_data["causal"].toBool(),
-                                             ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble());
+      auto [dq, dk, dv] = BackwardOp::call(g[0], s[0], s[1], s[2], s[3], s[4], s[5], if_defined(s[6]), if_defined(s[7]),
+                                    ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+                                    ctx->saved_data["cap"].toDouble());
       d = {dq, dk, dv};
     }
     d = once(std::move(d), {s[0], s[1], s[2], g[0]});
@@ -441,16 +483,21 @@ struct Attention : public torch::autograd::Function<Attention> {
   }
 };
 
-at::Tensor attention_train(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
-                           const OptTensor& slopes, bool causal, double scale, double cap) {
-  return Attention::apply(q, k, v, plan, slopes, causal, scale, cap);
+at::Tensor attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
+                              const OptTensor& slopes, bool causal, double scale, double cap) {
+  no_tangents({q, k, v, slopes});
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return Attention::apply(q, k, v, plan, slopes, causal, scale, cap);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return ForwardOp::call(q, k, v, plan, slopes, causal, scale, cap);
 }
 
 struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
                                const OptTensor& wq, const OptTensor& wk, const OptTensor& positions, double eps,
                                bool interleaved) {
-    auto [oq, ok] = rotary_forward(q, k, freq, wq, wk, positions, eps, interleaved);
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [oq, ok] = RotaryOp::call(q, k, freq, wq, wk, positions, eps, interleaved);
     ctx->save_for_backward({q, k, freq, or_undefined(wq), or_undefined(wk), or_undefined(positions)});
     ctx->saved_data["want_q"] = has(wq) && wq->requires_grad();
     ctx->saved_data["want_k"] = has(wk) && wk->requires_grad();
@@ -464,9 +511,9 @@ struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
     variable_list d;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dq, dk, dw] = rotary_backward(g[0], g[1], s[0], s[1], s[2], if_defined(s[3]), if_defined(s[4]),
-                                          if_defined(s[5]), ctx->saved_data["eps"].toDouble(),
-                                          ctx->saved_data["interleaved"].toBool(), want_q || want_k);
+      auto [dq, dk, dw] = RotaryBackwardOp::call(g[0], g[1], s[0], s[1], s[2], if_defined(s[3]), if_defined(s[4]), if_defined(s[5]),
+                                    ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(),
+                                    want_q || want_k);
       d = {dq, dk, want_q ? dw.select(0, 0).to(s[3].scalar_type()) : at::Tensor(),
            want_k ? dw.select(0, 1).to(s[4].scalar_type()) : at::Tensor()};
     }
@@ -478,32 +525,67 @@ struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
   }
 };
 
-std::tuple<at::Tensor, at::Tensor> rotary_train(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
-                                                const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
-                                                double eps, bool interleaved) {
-  auto out = QkNormRotary::apply(q, k, freq, wq, wk, positions, eps, interleaved);
-  return {out[0], out[1]};
+std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& freq,
+                                                   const OptTensor& wq, const OptTensor& wk, const OptTensor& positions,
+                                                   double eps, bool interleaved) {
+  no_tangents({q, k, freq, wq, wk});
+  const auto wants = [](const OptTensor& t) { return has(t) && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wants(wq) || wants(wk))) {
+    auto out = QkNormRotary::apply(q, k, freq, wq, wk, positions, eps, interleaved);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return RotaryOp::call(q, k, freq, wq, wk, positions, eps, interleaved);
 }
 
 }  // namespace
 
+TORCH_LIBRARY(bitscom_b200, m) {
+  m.def("attention_plan(Tensor? documents, Tensor? prefix, bool causal, int batch, int q_len, int k_len) -> Tensor");
+  m.def(
+      "attention_forward(Tensor q, Tensor k, Tensor v, Tensor? plan, Tensor? slopes, bool causal, float scale, "
+      "float cap) -> Tensor");
+  m.def(
+      "attention_forward_sums(Tensor q, Tensor k, Tensor v, Tensor? plan, Tensor? slopes, bool causal, float scale, "
+      "float cap) -> (Tensor out, Tensor sums, Tensor low)");
+  m.def(
+      "attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor out, Tensor sums, Tensor low, Tensor? plan, "
+      "Tensor? slopes, bool causal, float scale, float cap) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "rotary_forward(Tensor q, Tensor k, Tensor frequencies, Tensor? q_weight, Tensor? k_weight, Tensor? positions, "
+      "float eps, bool interleaved) -> (Tensor, Tensor)");
+  m.def(
+      "rotary_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor frequencies, Tensor? q_weight, "
+      "Tensor? k_weight, Tensor? positions, float eps, bool interleaved, bool want_gains) -> (Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(bitscom_b200, CUDA, m) {
+  m.impl("attention_plan", &attention_plan);
+  m.impl("attention_forward", &attention_forward);
+  m.impl("attention_forward_sums", &attention_forward_sums);
+  m.impl("attention_backward", &attention_backward);
+  m.impl("rotary_forward", &rotary_forward);
+  m.impl("rotary_backward", &rotary_backward);
+}
+
+TORCH_LIBRARY_IMPL(bitscom_b200, Autograd, m) {
+  m.impl("attention_forward", &attention_autograd);
+  m.impl("rotary_forward", &rotary_autograd);
+}
+
 void register_attention_bindings(pybind11::module_& m) {
   namespace py = pybind11;
-  m.def("attention_plan", &attention_plan, py::arg("documents"), py::arg("prefix"), py::arg("causal"), py::arg("batch"),
+  m.def("attention_plan", &PlanOp::call, py::arg("documents"), py::arg("prefix"), py::arg("causal"), py::arg("batch"),
         py::arg("q_len"), py::arg("k_len"));
-  m.def("attention_forward", &attention_forward, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"),
-        py::arg("slopes"), py::arg("causal"), py::arg("scale"), py::arg("cap"), py::arg("want_lse"));
-  m.def("attention_train", &attention_train, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("slopes"),
-        py::arg("causal"), py::arg("scale"), py::arg("cap"));
+  m.def("attention_forward", &ForwardOp::call, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"),
+        py::arg("slopes"), py::arg("causal"), py::arg("scale"), py::arg("cap"));
+  m.def("rotary_forward", &RotaryOp::call, py::arg("q"), py::arg("k"), py::arg("frequencies"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
   m.def("attention_status", [](bool reset) { return launch::attention_status(reset); }, py::arg("reset") = false,
         "1 once a wait of a tensor-core attention kernel on the current device ran out, else 0 (waits for the device).");
   m.def("attention_wait_limit", &launch::attention_wait_limit, py::arg("clocks"),
         "Sets how many clocks a wait inside a tensor-core attention kernel may last before the kernel gives up (0: the "
         "wait for scores always runs out, for tests of that path); returns the limit before.");
-  m.def("rotary_forward", &rotary_forward, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
-        py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
-  m.def("rotary_train", &rotary_train, py::arg("q"), py::arg("k"), py::arg("freq"), py::arg("wq"), py::arg("wk"),
-        py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
 }
 
 }  // namespace bitscom_b200

@@ -5,6 +5,7 @@ Needs a CUDA device."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import bitscom_b200 as bitscom
 from bitscom_b200 import _ext
@@ -164,3 +165,72 @@ def test_slopes_of_any_stride(cuda):
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (q, k, v), do), grads))
     same = bitscom.attention(q, k, v, slopes=slopes[:1].expand(4))
     assert torch.equal(same, bitscom.attention(q, k, v, slopes=torch.full((4,), 0.5, device="cuda")))
+
+
+def _traced_calls():
+    freq = bitscom.rotary_frequencies(64, device="cuda")
+    slopes = torch.tensor([0.5, 0.25], device="cuda")
+    gain = torch.linspace(0.5, 1.5, 64, device="cuda")
+    ids = torch.zeros(1, 150, dtype=torch.int32, device="cuda")
+    ids[:, 70:] = 1
+    return [
+        lambda q, k, v: bitscom.attention(q, k, v, softcap=5.0, slopes=slopes),
+        lambda q, k, v: bitscom.attention(q, k, v, documents=ids),
+        lambda q, k, v: bitscom.qk_norm_rotary(q.transpose(1, 2), k.transpose(1, 2), freq, q_weight=gain)[0],
+    ]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_traces_hold_the_kernels(cuda, which):
+    """A trace replayed on other inputs computes them: torch.jit.trace, and make_fx without and with a backward pass."""
+    f = _traced_calls()[which]
+    a, b = (_qkv(1, 2, 2, 150, 150, 64, torch.float16, seed=s) for s in (0, 1))
+
+    def with_grads(q, k, v, do):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = f(*leaves)
+        g = torch.autograd.grad(out, leaves, do if out.shape == do.shape else do.transpose(1, 2), allow_unused=True)
+        return (out.detach(), *(x for x in g if x is not None))
+
+    traced = torch.jit.trace(f, a[:3], check_trace=False)
+    torch.cuda.empty_cache()
+    assert torch.equal(traced(*b[:3]), f(*b[:3]))
+    graph = make_fx(f)(*a[:3])
+    assert torch.equal(graph(*b[:3]), f(*b[:3]))
+    for mode in ("real", "fake"):
+        graph = make_fx(with_grads, tracing_mode=mode, _allow_non_fake_inputs=True)(*a)
+        assert all(torch.equal(x, y) for x, y in zip(graph(*b), with_grads(*b)))
+
+
+@pytest.mark.parametrize("options", [dict(rotary=True, softcap=5.0), dict(distance_bias=True)], ids=str)
+def test_compiled_in_one_graph(cuda, options):
+    torch.manual_seed(0)
+    model = gpt2_small_test(vocab_size=64, n_positions=200, **options).cuda()
+    idx = torch.randint(0, 64, (2, 150), device="cuda")
+    ids = torch.arange(150, device="cuda").div(60, rounding_mode="floor").repeat(2, 1)
+
+    def run(m):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out = m(idx, documents=ids)
+        return [out.detach(), *torch.autograd.grad(out.float().square().mean(), list(model.parameters()))]
+
+    want = run(model)
+    torch._dynamo.reset()
+    got = run(torch.compile(model, backend="aot_eager", fullgraph=True))
+    # The same kernels on the same tensors; torch's embedding gradient adds with atomics.
+    assert torch.equal(got[0], want[0])
+    assert all(float((x - y).norm()) <= 1e-5 * float(y.norm()) for x, y in zip(got, want))
+
+
+def test_function_transforms(cuda):
+    """vmap runs the operators entry by entry; derivatives by transforms are refused."""
+    q, k, v, _ = _qkv(3, 2, 2, 40, 40, 64, torch.float16)
+    freq = bitscom.rotary_frequencies(64, device="cuda")
+    each = [x[:, None] for x in (q, k, v)]
+    assert torch.equal(torch.vmap(bitscom.attention)(*each)[:, 0], bitscom.attention(q, k, v))
+    got = torch.vmap(lambda a, b: bitscom.qk_norm_rotary(a, b, freq))(*each[:2])
+    assert all(torch.equal(x[:, 0], y) for x, y in zip(got, bitscom.qk_norm_rotary(q, k, freq)))
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda x: bitscom.attention(x, k, v).float().sum())(q)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda x: bitscom.qk_norm_rotary(x, k, freq)[0].float().sum())(q)
