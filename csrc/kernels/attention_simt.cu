@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(kThreads) keys_kernel(const AttnParams p) {
   }
 }
 
-// delta = sum over d of dout * o, one warp a row; o with what its rounding took, where that was kept.
+// delta = sum over d of dout * o, one warp a row.  In 16 bits o is the rounded result: delta is off by up to half a
+// step of sum |dout| |o|, beside the half step that every gradient is rounded by.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) delta_kernel(const AttnParams p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
@@ -291,10 +292,9 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const AttnParams p) {
   const int i = row % p.sq, h = row / p.sq % p.hq, b = row / (static_cast<int64_t>(p.sq) * p.hq);
   const T* o = static_cast<const T*>(p.o.ptr) + b * p.o.sb + h * p.o.sh + i * p.o.ss;
   const T* g = static_cast<const T*>(p.dout.ptr) + b * p.dout.sb + h * p.dout.sh + i * p.dout.ss;
-  const T* lo = p.lo.ptr != nullptr ? static_cast<const T*>(p.lo.ptr) + (o - static_cast<const T*>(p.o.ptr)) : nullptr;
   float sum = 0.f;
   for (int c = threadIdx.x & 31; c < p.d; c += 32)
-    sum += (to_f32<T>(o[c]) + (lo != nullptr ? to_f32<T>(lo[c]) : 0.f)) * to_f32<T>(g[c]);
+    sum += to_f32<T>(o[c]) * to_f32<T>(g[c]);
   for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   if ((threadIdx.x & 31) == 0) p.delta[row] = sum;
 }

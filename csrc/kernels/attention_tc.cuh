@@ -94,13 +94,13 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreScale& sc) 
 }
 
 // s = s * factor - slope |d0 + c| for N scores whose distances are d0, d0 + 1, ...  `slope`: of the
-// bias times log2 e; `side`: -1 when no distance is positive, 1 when none is negative, 0 when both occur.
+// bias times log2 e; `behind`: no distance is positive.
 template <int N>
-__device__ __forceinline__ void bias_scores(float (&s)[N], float factor, float slope, float d0, int side) {
-  if (side != 0) {
-    const float t = side < 0 ? slope : -slope, base = t * d0;  // the column is an immediate operand
+__device__ __forceinline__ void bias_scores(float (&s)[N], float factor, float slope, float d0, bool behind) {
+  if (behind) {
+    const float base = slope * d0;  // the column is an immediate operand
 #pragma unroll
-    for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, fmaf(t, static_cast<float>(c), base));
+    for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, fmaf(slope, static_cast<float>(c), base));
   } else {
 #pragma unroll
     for (int c = 0; c < N; ++c) s[c] = fmaf(s[c], factor, -slope * fabsf(d0 + c));

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 2)
       if (MODE == kCapped) cap_scores(s, fp.sc);
       if (MODE == kBiased || (MODE == kCapped && slope != 0.f)) {
         const bool behind = __all_sync(0xffffffffu, key0 + kCols - 1 <= pos);
-        bias_scores(s, MODE == kBiased ? fp.sc.c : 1.f, slope, static_cast<float>(key0 - pos), behind ? -1 : 0);
+        bias_scores(s, MODE == kBiased ? fp.sc.c : 1.f, slope, static_cast<float>(key0 - pos), behind);
       }
       if (!(tr.z <= key0 && tr.w >= key0 + kCols)) {
         const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
