@@ -234,3 +234,48 @@ def test_function_transforms(cuda):
         torch.func.grad(lambda x: bitscom.attention(x, k, v).float().sum())(q)
     with pytest.raises(RuntimeError, match="functorch"):
         torch.func.grad(lambda x: bitscom.qk_norm_rotary(x, k, freq)[0].float().sum())(q)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_score_gradients_do_not_see_the_outputs_rounding(cuda, dtype, d):
+    """delta = do.o takes o as it was before its rounding.
+
+    Queries of zero make every weight 1/16, which no type rounds, and values near 8 make o.do large beside
+    do.(v - o), so that half a step of o in delta would show.  Left are: ds rounded once, o kept in two values of
+    the type (a half step of a half step), and fp32 sums of d and 16 terms, at most (2 * 16 + d + 16) roundings of 2^-24
+    of sum |do| |v|.  Each goes into dq with weight |k|, and dq is rounded once.
+    """
+    u, sk = torch.finfo(dtype).eps / 2, 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.zeros(1, 2, 200, d, device="cuda", dtype=dtype, requires_grad=True)
+    k, v = ((m + f * torch.randn(1, 2, sk, d, generator=g, device="cuda")).to(dtype) for m, f in ((1, 0.1), (8, 0.25)))
+    do = torch.randn(1, 2, 200, d, generator=g, device="cuda").to(dtype)
+    (dq,) = torch.autograd.grad(bitscom.attention(q, k, v, causal=False), q, do)
+    kd, vd, dod = (x.double() for x in (k, v, do))
+    o = vd.mean(2, keepdim=True)
+    ds = (dod @ (vd - o).transpose(-1, -2)) / sk
+    want = ds @ kd * d ** -0.5
+    ado = (dod.abs() @ vd.abs().transpose(-1, -2)) / sk
+    e = 2.0 ** -24 * (2 * sk + d + 16)
+    step = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half of fp16's smallest step
+    bound = ((u + e) * ds.abs() + (u * u + e) * ado + step) @ kd.abs() * d ** -0.5 + u * want.abs() + step
+    assert ((dq.double() - want).abs() <= 1.05 * bound).all()
+    # A delta from the rounded output is beyond it: the test can tell.
+    off = ((o.to(dtype).double() - o) * dod).sum(-1, keepdim=True) / sk
+    assert ((off * kd.sum(2, keepdim=True) * d ** -0.5).abs() > 1.05 * bound).any()
+
+
+@pytest.mark.parametrize("sq,sk", [(1, 300), (3, 2600), (17, 1100)])
+@pytest.mark.parametrize("heads", [(8, 2), (6, 6)], ids=str)
+def test_few_queries_over_packed_documents(cuda, heads, sq, sk):
+    """Shared heads in one tile and key splits, with documents, padding on the left and prefixes."""
+    ids = torch.zeros(2, sk, dtype=torch.int32)
+    ids[0, : sk // 3] = -1
+    ids[1, sk - 2 :] = 4  # the last queries are alone, the first of 17 see the long document
+    for d, dtype, cap in ((64, torch.bfloat16, None), (128, torch.float16, 20.0), (128, torch.bfloat16, None)):
+        q, k, v, do = _qkv(2, *heads, sq, sk, d, dtype, seed=sk)
+        for prefix in (None, torch.tensor([sk // 2, sk])):
+            out = bitscom.attention(q, k, v, documents=ids.cuda(), prefix=None if prefix is None else prefix.cuda(), softcap=cap)
+            vals, bounds = reference(q, k, v, do, seen=visible(2, sq, sk, True, ids, prefix), softcap=cap)
+            check({"out": out}, vals, bounds)
