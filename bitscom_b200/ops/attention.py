@@ -125,7 +125,7 @@ def attention(
         documents, prefix: see the module's description and
             :func:`attention_mask`, which builds them into a ``mask`` once for
             several calls; ``mask`` replaces ``causal``, ``documents``, ``prefix``.
-        softcap: cap of the scores (1e-30 to 1e30), None for none.
+        softcap: cap of the scores (1e-12 to 1e30), None for none.
         slopes: ``[heads]`` distance slopes (not differentiated).
         scale: factor of ``q.k`` (1e-30 to 1e30), default ``head size ** -0.5``.
 
@@ -141,8 +141,8 @@ def attention(
     """
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k and v must be [batch, heads, length, head size]")
-    if softcap is not None and not 1e-30 <= softcap <= 1e30:
-        raise ValueError(f"softcap must be positive, from 1e-30 to 1e30, got {softcap}")
+    if softcap is not None and not 1e-12 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be positive, from 1e-12 to 1e30, got {softcap}")
     if scale is not None and not 1e-30 <= scale <= 1e30:
         raise ValueError(f"scale must be positive, from 1e-30 to 1e30, got {scale}")
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 #include "attention_common.cuh"
 #include "tcgen05.cuh"
@@ -29,6 +30,9 @@ struct ScoreScale {
   float cap_in;   // capped: 2 log2 e * scale / cap
   float cap_out;  // capped: cap * log2 e
   float cap_inv;  // capped: 1 / cap_out
+  // A masked score of the backward pass.  Under a cap it is finite, and so is the square of masked * cap_inv in the
+  // factor 1 - tanh^2, which a weight of zero then makes zero; the weight is zero for every accepted cap (from 1e-12 on).
+  float masked;
   float near, mid;          // capped: largest raw scores of the polynomials, -1: not used
   float poly3[3], poly5[5];  // capped: the polynomials for raw scores, times cap_out
   // In double, as powers of scale / cap leave the range of fp32 for caps that are accepted.
@@ -37,11 +41,13 @@ struct ScoreScale {
     constexpr double square = 1e18;                 // what the polynomials can square
     ScoreScale s{};
     s.c = p.scale * kLog2e;
+    s.masked = -INFINITY;
     if (p.cap > 0.f) {
       const double k = static_cast<double>(p.scale) / p.cap, out = static_cast<double>(p.cap) * kLog2e;
       s.cap_out = static_cast<float>(out);
       s.cap_in = static_cast<float>(std::min(2. * kLog2e * k, most));
       s.cap_inv = static_cast<float>(1. / out);
+      s.masked = static_cast<float>(-std::min(1e15, 1e18 * out));
       s.near = static_cast<float>(std::min(kTanhNear / k, square));
       s.mid = static_cast<float>(std::min(kTanhMid / k, square));
       double f = k * out;

@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Pair nlse2(nlse, nlse), delta2(-delta, -delta), c2(bp.sc.c, bp.sc.c);
     const Pair inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
     const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
+    const float masked = MODE == kCapped ? bp.sc.masked : -INFINITY;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
     for (int j = 0; j < n; ++j) {
       const int key0 = (t0 + j) * kAttnTile + part * kPart;
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!full) {
         const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
 #pragma unroll
-        for (int c = 0; c < kPart; ++c) pf[c] = from + c < len ? pf[c] : -INFINITY;
+        for (int c = 0; c < kPart; ++c) pf[c] = from + c < len ? pf[c] : masked;
       }
       const float d0 = static_cast<float>(key0 - pos);
       // The distance's sign is known (masked pairs do not count): the bias joins the log-sum.
@@ -361,11 +362,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float x = fmaf(pf[c], MODE == kCapped ? 1.f : bp.sc.c, fmaf(-slope, fabsf(d0 + c), nlse));
           pf[c] = ex2(x) * (f * prob_unshift<T>());
         }
-      }
-      if (MODE == kCapped && !full) {  // of a masked pair, zero times an infinite 1 - tanh^2
-        const unsigned len = static_cast<unsigned>(range.y - range.x), from = static_cast<unsigned>(key0 - range.x);
-#pragma unroll
-        for (int c = 0; c < kPart; ++c) pf[c] = from + c < len ? pf[c] : 0.f;
       }
       if (!(ok = guard.wait_warp(&bar.dp_full, j & 1))) break;
       tc_fence_after();
@@ -643,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int key = key0 + r;
     const Pair c2(bp.sc.c, bp.sc.c), inv2(bp.sc.cap_inv, bp.sc.cap_inv), one2(1.f, 1.f), minus2(-1.f, -1.f);
     const Pair unshift2(prob_unshift<T>(), prob_unshift<T>());
+    const float masked = MODE == kCapped ? bp.sc.masked : -INFINITY;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
     bool more = some;
     int j = 0;
@@ -666,12 +663,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kPart; c += 2) {
             const int4 v = *reinterpret_cast<const int4*>(range + c);
-            pf[c] = key >= v.x && key < v.y ? pf[c] : -INFINITY;
-            pf[c + 1] = key >= v.z && key < v.w ? pf[c + 1] : -INFINITY;
+            pf[c] = key >= v.x && key < v.y ? pf[c] : masked;
+            pf[c + 1] = key >= v.z && key < v.w ? pf[c + 1] : masked;
           }
         } else if (p.causal) {  // rows from position `key` on
 #pragma unroll
-          for (int c = 0; c < kPart; ++c) pf[c] = c >= key - first_pos ? pf[c] : -INFINITY;
+          for (int c = 0; c < kPart; ++c) pf[c] = c >= key - first_pos ? pf[c] : masked;
         }
       }
       uint32_t w[kPart / 2];
@@ -709,19 +706,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (prob_unshift<T>() != 1.f) f = mul2(f, unshift2);
           f.split(pf[c + e], pf[c + e + 1]);
-        }
-      }
-      if (MODE == kCapped && !full) {  // of a masked pair, zero times an infinite 1 - tanh^2
-        if (p.plan.range != nullptr) {
-#pragma unroll
-          for (int c = 0; c < kPart; c += 2) {
-            const int4 v = *reinterpret_cast<const int4*>(range + c);
-            pf[c] = key >= v.x && key < v.y ? pf[c] : 0.f;
-            pf[c + 1] = key >= v.z && key < v.w ? pf[c + 1] : 0.f;
-          }
-        } else if (p.causal) {
-#pragma unroll
-          for (int c = 0; c < kPart; ++c) pf[c] = c >= key - first_pos ? pf[c] : 0.f;
         }
       }
       if (kOwn && j > 0) {  // the last P has been read

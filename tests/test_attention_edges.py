@@ -15,7 +15,7 @@ def test_caps_and_scales_outside_fp32_are_refused():
             bitscom.attention(q, k, v, softcap=bad)
         with pytest.raises(ValueError):
             bitscom.attention(q, k, v, scale=bad)
-    for cap in (1e-30, 1e30):
+    for cap in (1e-12, 1e30):
         assert torch.isfinite(bitscom.attention(q, k, v, softcap=cap)).all()
 
 

@@ -78,7 +78,7 @@ def test_shared_memory_of_another_call_does_not_show(cuda, dtype):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
-@pytest.mark.parametrize("cap", [1e-3, 1e-5, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("cap", [1e-3, 1e-5, 1e-8, 1e-12])
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64)], ids=str)
 def test_caps_far_below_the_scores(cuda, dtype, d, cap):
     """Scores of +-cap: nearly even weights, and no gradient through the scores but where one is near zero."""
