@@ -136,7 +136,8 @@ def attention(
     any other key can reach every query whose tile of 128 keys holds it.
     Gradients are by the backward pass, once; on CUDA a forward-mode tangent is refused.
     float16 and bfloat16 round the probabilities and score gradients to that
-    type for the products; all sums are float32.  Under autocast float32 inputs
+    type for the products (in float16 score gradients below 6e-5 lose bits: scale
+    the loss); all sums are float32.  Under autocast float32 inputs
     are cast like those of torch's own attention.
     """
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:

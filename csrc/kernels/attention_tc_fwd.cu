@@ -11,17 +11,17 @@
 //
 // S has two places in TMEM: the scores of the tile after next are formed when this
 // tile's P has been read, so the softmax warps find theirs ready.  D = 64 keeps Q in TMEM
-// as well: an instruction with one operand in shared memory takes 44 clocks
-// for 64 keys, with two 74.  Two CTAs share an SM (256 TMEM columns each), one's start
-// and end beside the other's work.
+// as well, which halves what S reads from shared memory.  Two CTAs share an SM (256 TMEM
+// columns each), one's start and end beside the other's work.
 //
 // What bounds it: a score costs one exponential, 16 a clock and SM, and 4 D
-// operations.  A tile of 64 keys takes a warp 1500 clocks, 700 of them exponentials, the
-// rest latency (TMEM load 80, maximum 100, two votes, TMEM store 60, barriers): two
-// warps a scheduler keep the exponential pipe busy about 60 % of the time.  16 heads x
-// 4096 rows, causal: D = 64 71 us (480 TFLOP/s), with distance bias 90 us; D = 128 91 us
-// (750 TFLOP/s, MMA bound: S with both operands in shared memory), capped 131 us.
-// A CTA costs 6000 to 7000 clocks besides its tiles.
+// operations.  No pipe is full: at D = 64 that of the exponentials is busy 59 % of the
+// time and the tensor cores 27 %, and warps wait most for instructions of fixed
+// latency (TMEM loads and stores, maxima, votes, barriers), which a tile of 64 keys pays
+// once.  16 heads x 4096 rows, causal: D = 64 60 us (570 TFLOP/s), with distance bias 88 us,
+// capped 95 us; D = 128 78 us (880 TFLOP/s), capped 104 us.  One query of 16 heads on 4 over 8
+// caches of 32768 x 128: 85 us, 92 % of a copy's bandwidth.  A CTA of three tiles alone takes
+// 6.8 us with its launch, so short rows are bound by start and end.
 //
 // The running maximum is only followed when it grows by more than 4 (a factor of
 // 16 in P), so most tiles do not touch O; the sum uses the same reference, so the

@@ -5,8 +5,9 @@
 //   (y1, y2) -> (y1 cos a - y2 sin a, y2 cos a + y1 sin a),  a = position * freq
 //   backward: g = dy turned by -a;  dw = sum g n;  dx = r (g w - n mean(g w n))
 //
-// Bound by memory: each head is read once and written once (backward: x and
-// dy read, dx written).  A head's D values lie in 16-byte pieces across a group
+// Each head is read once and written once (backward: x and dy read, dx written).  Long
+// rows are bound by memory with too few loads in flight; what fits in L2 (8 x 1024 tokens x 32
+// heads x 64) by the instructions of a token's angles and heads, issuing on half of all clocks.  A head's D values lie in 16-byte pieces across a group
 // of 8, 16 or 32 lanes, so the norm is a few shuffles; the partner of a pair
 // (i, i + rotated / 2) sits in another lane at the same place of its piece, one
 // shuffle more.  When a half is not a whole number of pieces, the partners are
@@ -19,7 +20,7 @@
 // heads' loads under way.  No lane group waits for another: with angles
 // formed by the block in shared memory and a head to a lane group, the barriers and the
 // divisions for each head held 131072 tokens x 20 heads x 128 (fp16) at 629 us; this
-// form takes 327 us (4.1 TB/s, 62 % of a copy).  Two blocks of 128
+// form takes 336 us (4.0 TB/s, 61 % of a copy).  Two blocks of 128
 // registers a thread an SM: three of 80 spill (452 us).
 //
 // The gains' gradients are summed in registers over a lane group's heads, then
