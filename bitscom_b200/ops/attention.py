@@ -234,23 +234,23 @@ if _ext.available():  # what tracing with fake tensors sees: the layouts of csrc
     def _tokens_first(t):
         return t.new_empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3])).transpose(1, 2)
 
-    @torch.library.register_fake("bitscom_b200::attention_plan")
+    @torch.library.register_fake("bitscom_b200::attention_plan", allow_override=True)
     def _(documents, prefix, causal, batch, q_len, k_len):
         like = documents if documents is not None else prefix
         q_tiles, k_tiles = (q_len + 127) // 128, (k_len + 127) // 128
         return like.new_empty(batch * (q_tiles * (2 * 128 + 8) + k_tiles * 4), dtype=torch.int32)
 
-    @torch.library.register_fake("bitscom_b200::attention_forward")
+    @torch.library.register_fake("bitscom_b200::attention_forward", allow_override=True)
     def _(q, k, v, plan, slopes, causal, scale, cap):
         return _tokens_first(q)
 
-    @torch.library.register_fake("bitscom_b200::attention_forward_sums")
+    @torch.library.register_fake("bitscom_b200::attention_forward_sums", allow_override=True)
     def _(q, k, v, plan, slopes, causal, scale, cap):
         tensor_cores = q.dtype != torch.float32 and q.shape[3] % 8 == 0 and q.shape[3] <= 128
         sums = q.new_empty(q.shape[:3], dtype=torch.float32)
         return _tokens_first(q), sums, _tokens_first(q) if tensor_cores else q.new_empty(0)
 
-    @torch.library.register_fake("bitscom_b200::attention_backward")
+    @torch.library.register_fake("bitscom_b200::attention_backward", allow_override=True)
     def _(grad, q, k, v, out, sums, low, plan, slopes, causal, scale, cap):
         return _tokens_first(q), _tokens_first(k), _tokens_first(v)
 

@@ -110,11 +110,11 @@ def _qk_norm_rotary_cpu(q, k, freq, wq, wk, positions, eps, interleaved):
 
 if _ext.available():  # what tracing with fake tensors sees
 
-    @torch.library.register_fake("bitscom_b200::rotary_forward")
+    @torch.library.register_fake("bitscom_b200::rotary_forward", allow_override=True)
     def _(q, k, frequencies, q_weight, k_weight, positions, eps, interleaved):
         return q.new_empty(q.shape), k.new_empty(k.shape)
 
-    @torch.library.register_fake("bitscom_b200::rotary_backward")
+    @torch.library.register_fake("bitscom_b200::rotary_backward", allow_override=True)
     def _(grad_q, grad_k, q, k, frequencies, q_weight, k_weight, positions, eps, interleaved, want_gains):
         gains = q.new_empty((2, q.shape[3]) if want_gains else (0,), dtype=torch.float32)
         return q.new_empty(q.shape), k.new_empty(k.shape), gains
