@@ -110,7 +110,12 @@ void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
 // As the kernels read them, which is one after another.
 OptTensor slopes_of(const OptTensor& t) { return has(t) ? OptTensor(t->contiguous()) : OptTensor(); }
 
-// The tensors have to outlive the launch: `slopes` is from slopes_of().
+// The kernels read a plan 16 bytes at a time.
+OptTensor plan_of(const OptTensor& t) {
+  return has(t) && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0 ? OptTensor(t->clone()) : t;
+}
+
+// The tensors have to outlive the launch: `plan` and `slopes` are from plan_of() and slopes_of().
 AttnParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& plan,
                      const OptTensor& slopes, bool causal, double scale, double cap) {
   AttnParams p{};
@@ -182,13 +187,13 @@ at::Tensor attention_plan(const OptTensor& documents, const OptTensor& prefix, b
 // Returns (out, log-sums, out's rounding); the last two only for the backward pass, the last one empty where
 // it is not kept.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> run_forward(const at::Tensor& q_in, const at::Tensor& k_in,
-                                                           const at::Tensor& v_in, const OptTensor& plan,
+                                                           const at::Tensor& v_in, const OptTensor& plan_in,
                                                            const OptTensor& slopes_in, bool causal, double scale,
                                                            double cap, bool want_sums) {
   check_qkv(q_in, k_in, v_in);
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
-  const OptTensor slopes = slopes_of(slopes_in);
+  const OptTensor plan = plan_of(plan_in), slopes = slopes_of(slopes_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   auto out = tokens_first(q);
   at::Tensor lse, lo;
@@ -235,17 +240,25 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward_sums(const at::
   return run_forward(q, k, v, plan, slopes, causal, scale, cap, true);
 }
 
+// What autograd hands back need not lie as it was saved (hooks that move saved tensors): out, low, sums and plan are
+// copied where their place does not fit.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     const at::Tensor& dout_in, const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
-    const at::Tensor& out, const at::Tensor& lse, const at::Tensor& lo, const OptTensor& plan,
+    const at::Tensor& out_in, const at::Tensor& lse_in, const at::Tensor& lo_in, const OptTensor& plan_in,
     const OptTensor& slopes_in, bool causal, double scale, double cap) {
   check_qkv(q_in, k_in, v_in);
   same_device(dout_in, q_in, "the output's gradient");
+  same_device(out_in, q_in, "the output");
+  same_device(lse_in, q_in, "the log-sums");
+  same_device(lo_in, q_in, "the output's rounding");
   c10::cuda::CUDAGuard g(q_in.device());
   const auto q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
-  const auto dout = rows_of(dout_in.to(q.scalar_type()));
-  TORCH_CHECK_VALUE(dout.sizes() == q.sizes() && out.sizes() == q.sizes(), "bitscom: the output's gradient must be ",
-                    q.sizes());
+  TORCH_CHECK_VALUE(dout_in.sizes() == q.sizes(), "bitscom: the output's gradient must be ", q.sizes());
+  TORCH_CHECK_VALUE(out_in.sizes() == q.sizes() && out_in.scalar_type() == q.scalar_type() &&
+                        lse_in.scalar_type() == at::kFloat && lse_in.sizes() == q.sizes().slice(0, 3),
+                    "bitscom: the output and its log-sums are not of these queries");
+  const auto dout = rows_of(dout_in.to(q.scalar_type())), out = rows_of(out_in);
+  const auto lse = lse_in.contiguous();
   auto dq = tokens_first(q), dk = tokens_first(k), dv = tokens_first(v);
   if (q.numel() == 0 || k.numel() == 0) {
     dq.zero_();
@@ -253,7 +266,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
     dv.zero_();
     return {dq, dk, dv};
   }
-  const OptTensor slopes = slopes_of(slopes_in);
+  const OptTensor plan = plan_of(plan_in), slopes = slopes_of(slopes_in);
   AttnParams p = params_of(q, k, v, plan, slopes, causal, scale, cap);
   p.o = view_of(out);
   p.dout = view_of(dout);
@@ -262,7 +275,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
   p.dv = view_of(dv);
   p.lse = lse.data_ptr<float>();
   if (for_tensor_cores(q)) {
-    TORCH_CHECK(lo.sizes() == out.sizes(), "bitscom: the forward pass kept no rounding of its output");
+    TORCH_CHECK_VALUE(lo_in.sizes() == out.sizes() && lo_in.scalar_type() == out.scalar_type(),
+                      "bitscom: the forward pass kept no rounding of its output");
+    auto lo = rows_of(lo_in);
+    if (lo.strides() != out.strides()) lo = at::empty_strided(out.sizes(), out.strides(), out.options()).copy_(lo);
     p.lo = view_of(lo);
     const int64_t tiles = (q.size(2) + kAttnTile - 1) / kAttnTile;
     auto stats = at::empty({q.size(0), q.size(1), tiles, 2, kAttnTile}, lse.options());

@@ -279,3 +279,30 @@ def test_few_queries_over_packed_documents(cuda, heads, sq, sk):
             out = bitscom.attention(q, k, v, documents=ids.cuda(), prefix=None if prefix is None else prefix.cuda(), softcap=cap)
             vals, bounds = reference(q, k, v, do, seen=visible(2, sq, sk, True, ids, prefix), softcap=cap)
             check({"out": out}, vals, bounds)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=str)
+def test_saved_tensors_may_come_back_elsewhere(cuda, dtype):
+    """Hooks that hand saved tensors back with other strides, or off their alignment, change nothing."""
+    q, k, v, do = _qkv(2, 4, 2, 150, 150, 64, dtype, grad=True)
+    ids = torch.arange(150, device="cuda").div(60, rounding_mode="floor").int().repeat(2, 1)
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    out = bitscom.attention(q, k, v, documents=ids, slopes=slopes)
+    want = torch.autograd.grad(out, (q, k, v), do)
+
+    def moved(t):  # one element further in memory
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+
+    def reordered(t):  # dimensions in the reverse order, the last one too
+        return t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))
+
+    count = [0]
+
+    def in_turn(t):
+        count[0] += 1
+        return (moved, reordered, torch.clone)[count[0] % 3](t)
+
+    for unpack in (moved, reordered, in_turn, in_turn):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = bitscom.attention(q, k, v, documents=ids, slopes=slopes)
+        assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(out, (q, k, v), do), want))
